@@ -292,6 +292,7 @@ __device__ __forceinline__ void fm_dense_final_body(const FmDenseFinalArgs& a, f
 // on the device and multiplies them by beta once per step; alpha_t is formed from them in fp32.
 // One thread calls this.
 __device__ __forceinline__ void adam_schedule_body(float* __restrict__ sched, float lr, float b1, float b2) {
+#pragma clang fp contract(off)  // 1 - power has to see the ROUNDED power, as the host's schedule (ops.TFAdamSchedule) does
   const float b1p = sched[1] * b1;
   const float b2p = sched[2] * b2;
   sched[1] = b1p;
