@@ -56,6 +56,7 @@ extern "C" {
 
 #define MI_DT_F32 0
 #define MI_DT_BF16 1
+#define MI_DT_E4M3 2 /* 8 bits: 4 of exponent, 3 of mantissa, no infinity; history caches only */
 
 const char* mi_version(void);
 const char* mi_last_error(void);
@@ -905,6 +906,56 @@ int mi_bce_logits(const float* logits, const float* labels, int64_t B, float gsc
  * for decode_csv; mi_last_error() names the line. */
 int mi_parse_records(const char* text, int64_t len, int n_fields, int bag_len, int64_t max_rows,
                      int32_t* scalars, int32_t* bags, int64_t* n_rows, int64_t* consumed);
+
+/* ------------------------------------------------------------------------------------
+ * User histories: a paged cache of keys and values on the device, appended event by event, read back, and attended
+ * by new tokens or candidates.  No counterpart in the reference, whose requests carry their whole (six-entry) history
+ * with them (r_model.py:68-80 pools it with equal weights); this is what a history too long for that needs.
+ *
+ * Pages hold page_size positions of ONE sequence; page_table[b][i] (int32, row stride ld_table, table_width pages of
+ * room) names the page of positions [i*page_size, (i+1)*page_size) of sequence b.  Sequences may share pages that
+ * nobody writes any more.  lengths[b] (int32) counts the positions of sequence b, those that the same step appends
+ * included; <= 0 is a sequence without history (padding of a batch).
+ * MI_IDERR_RANGE is raised for a page id outside [0, n_pages) where a position needs it and for a length beyond
+ * table_width*page_size; such positions are skipped (write), zeros (read), absent (attention).
+ * ---------------------------------------------------------------------------------- */
+typedef struct mi_hist_cache {
+  void* kv;        /* [n_pages][n_heads][2][page_size][dim], 0 keys, 1 values; 16-byte aligned */
+  uint8_t* exps;   /* e4m3 only: [n_pages][n_heads][2][page_size]; a row stands for code * 2^(exps - 127) */
+  int64_t n_pages;
+  int n_heads;
+  int page_size;   /* a power of two, 16..1024 */
+  int dim;         /* 32, 64, 128 or 256 */
+  int dtype;       /* MI_DT_F32, MI_DT_BF16 or MI_DT_E4M3 */
+} mi_hist_cache;
+
+/* Appends rows: the n_b rows that sequence b owns are its newest positions, row i of them position
+ * lengths[b] - n_b + i.  Sequence b owns rows [offsets[b], offsets[b+1]) (int64 [n_seqs+1], ascending), or with
+ * offsets == NULL n_rows/n_seqs rows each.  Rows nobody owns and rows in front of position 0 are ignored.  k, v: rows
+ * of n_heads * dim values, f32 or bf16, row and head strides in elements, 16-byte aligned.  Stored rounded to nearest
+ * even; in e4m3 with the row's smallest exponent e >= -126 for which max finite |x| * 2^-e <= 448, infinities and NaN
+ * as NaN.  A page that receives positions must stand in one place of the table only. */
+int mi_hist_write(const mi_hist_cache* cache, const void* k, const void* v, int dtype, int64_t k_row, int64_t k_head,
+                  int64_t v_row, int64_t v_head, int64_t n_rows, const int64_t* offsets, int64_t n_seqs,
+                  const int32_t* page_table, int64_t ld_table, int table_width, const int32_t* lengths,
+                  int32_t* err, void* stream);
+
+/* The mirror image: k, v (f32 or bf16) = the newest positions, packed by the same rule.  Rows nobody owns are left as
+ * they are; rows without a place in the cache (in front of position 0, bad page) become zeros. */
+int mi_hist_read(const mi_hist_cache* cache, void* k, void* v, int dtype, int64_t k_row, int64_t k_head, int64_t v_row,
+                 int64_t v_head, int64_t n_rows, const int64_t* offsets, int64_t n_seqs, const int32_t* page_table,
+                 int64_t ld_table, int table_width, const int32_t* lengths, int32_t* err, void* stream);
+
+/* Attention of n_queries new tokens (or candidates) of every sequence over ALL lengths[b] positions of its history:
+ *   out[b][t][h] = sum_j softmax_j(scale * <q[b][t][h], k_j>) v_j,   k_j, v_j of cache head h / (q_heads / n_heads).
+ * Queries of one sequence do not see each other.  A row without a position of finite score gives zeros.  q, out:
+ * f32 for an f32 cache, bf16 otherwise; sequence, token and head strides in elements, 16-byte aligned.  Sums and
+ * softmax statistics in f32. */
+size_t mi_hist_attn_workspace_bytes(const mi_hist_cache* cache, int64_t n_seqs, int n_queries, int q_heads, int table_width);
+int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q_seq, int64_t q_tok, int64_t q_head, int q_heads,
+                 int n_queries, int64_t n_seqs, const int32_t* page_table, int64_t ld_table, int table_width,
+                 const int32_t* lengths, float scale, void* out, int64_t out_seq, int64_t out_tok, int64_t out_head,
+                 void* workspace, size_t workspace_bytes, int32_t* err, void* stream);
 
 #ifdef __cplusplus
 }

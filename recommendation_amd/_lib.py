@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get('MI355REC_LIB') or os.path.join(_HERE, 'libmi355rec.so
 MI_CHECK_RANGE, MI_CHECK_INCREASING, MI_CHECK_NONNEG = 1, 2, 4
 MI_IDERR_RANGE, MI_IDERR_ORDER, MI_IDERR_INTERNAL, MI_IDERR_CAPACITY = 1, 2, 4, 8
 MI_POOL_SUM, MI_POOL_MEAN = 0, 1
-MI_DT_F32, MI_DT_BF16 = 0, 1
+MI_DT_F32, MI_DT_BF16, MI_DT_E4M3 = 0, 1, 2
 MI_OPT_SGD, MI_OPT_ADAGRAD_ROWWISE, MI_OPT_ADAM_TF = 0, 1, 2
 MI_NOALLOC_MAX_ENTRIES = 1 << 21
 MI_COMM_ID_BYTES = 128
@@ -75,6 +75,12 @@ class GemmEpilogue(Structure):
     _fields_ = [('mode', c_int), ('flags', c_int), ('out', c_void_p), ('ld_out', c_int64), ('bias', c_void_p),
                 ('in0', c_void_p), ('ld_in0', c_int64), ('in1', c_void_p), ('ld_in1', c_int64),
                 ('out1', c_void_p), ('ld_out1', c_int64), ('bias_ld', c_int64), ('bias_rows', c_int)]
+
+
+class HistCacheC(Structure):
+    """mi_hist_cache"""
+    _fields_ = [('kv', c_void_p), ('exps', c_void_p), ('n_pages', c_int64), ('n_heads', c_int), ('page_size', c_int),
+                ('dim', c_int), ('dtype', c_int)]
 
 
 P = c_void_p
@@ -191,6 +197,13 @@ _SIGNATURES = {
     'mi_a2a_pooled': (c_int, [P, P, P, c_int64, P]),
     'mi_allgather_bytes': (c_int, [P, P, P, c_int64, P]),
     'mi_allreduce_dense': (c_int, [P, P, c_int64, P]),
+    'mi_hist_write': (c_int, [POINTER(HistCacheC), P, P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, P, c_int64, P,
+                              c_int64, c_int, P, P, P]),
+    'mi_hist_read': (c_int, [POINTER(HistCacheC), P, P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, P, c_int64, P,
+                             c_int64, c_int, P, P, P]),
+    'mi_hist_attn_workspace_bytes': (c_size_t, [POINTER(HistCacheC), c_int64, c_int, c_int, c_int]),
+    'mi_hist_attn': (c_int, [POINTER(HistCacheC), P, c_int64, c_int64, c_int64, c_int, c_int, c_int64, P, c_int64, c_int, P,
+                             c_float, P, c_int64, c_int64, c_int64, P, c_size_t, P, P]),
     'mi_fm_dense_step_rows': (c_int, [P, c_int, c_int, c_int, c_int64, P, P, P, c_float, P, c_float, c_float,
                                       c_float, P, P]),
 }

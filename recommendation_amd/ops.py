@@ -8,7 +8,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import (MI_CHECK_INCREASING, MI_CHECK_NONNEG, MI_CHECK_RANGE, MI_DT_BF16, MI_DT_F32,
+from ._lib import (MI_CHECK_INCREASING, MI_CHECK_NONNEG, MI_CHECK_RANGE, MI_DT_BF16, MI_DT_E4M3, MI_DT_F32,
                    MI_IDERR_CAPACITY, MI_IDERR_ORDER, MI_IDERR_RANGE, MI_OPT_ADAGRAD_ROWWISE, MI_OPT_ADAM_TF, MI_OPT_SGD,
                    MI_POOL_MEAN, MI_POOL_SUM, BwdPlan, MiError)
 
@@ -995,3 +995,148 @@ class DinUnit(object):
     def backward(self, feat, dfeat, ids_all, dE, beta1, beta2, eps, lr_t=0.0, lr_dev=None):
         _lib.call('mi_din_lau_bwd', ctypes.byref(self.c), self.B, _p(self.ws), self.ws.numel(), _p(feat), feat.stride(0),
                   _p(dfeat), dfeat.stride(0), _p(ids_all), lr_t, _p(lr_dev), beta1, beta2, eps, _p(dE), _stream())
+
+
+# ----------------------------------------------------------------------------- user histories (paged keys and values)
+class HistCache(object):
+    """struct mi_hist_cache: pages of keys and values, ``kv`` [n_pages, n_heads, 2, page_size, dim] (0 keys, 1 values) in
+    float32, bfloat16 or float8_e4m3fn; an 8-bit cache has ``exps`` [n_pages, n_heads, 2, page_size] beside it (a row
+    stands for code * 2^(exps - 127)).  Which page holds which positions of which sequence is the caller's table."""
+
+    _DTYPES = {torch.float32: MI_DT_F32, torch.bfloat16: MI_DT_BF16, torch.float8_e4m3fn: MI_DT_E4M3}
+
+    def __init__(self, n_pages, page_size, n_heads, dim, dtype=torch.bfloat16, device=None, kv=None, exps=None):
+        """``kv`` (and ``exps``): existing storage to use, otherwise it is allocated on ``device`` and left unset."""
+        if dtype not in self._DTYPES:
+            raise TypeError("HistCache: dtype must be float32, bfloat16 or float8_e4m3fn, got %s" % dtype)
+        shape = (int(n_pages), int(n_heads), 2, int(page_size), int(dim))
+        if min(shape) < 1:
+            raise MiError("HistCache: sizes must be positive, got %s" % (shape,))
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise MiError("HistCache: page_size %d is not a power of two from 16 to 1024" % page_size)
+        if dim not in (32, 64, 128, 256):
+            raise MiError("HistCache: dim %d is not 32, 64, 128 or 256" % dim)
+        if kv is None:
+            if exps is not None:
+                raise MiError("HistCache: exps without kv")
+            kv = torch.empty(shape, dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype, device=device).view(dtype)
+        if tuple(kv.shape) != shape or kv.dtype != dtype or not kv.is_contiguous():
+            raise MiError("HistCache: kv must be a contiguous %s tensor of shape %s" % (dtype, shape))
+        if dtype != torch.float8_e4m3fn:
+            if exps is not None:
+                raise MiError("HistCache: only 8-bit caches have exps")
+        elif exps is None:
+            exps = torch.empty(shape[:-1], dtype=torch.uint8, device=kv.device)
+        elif tuple(exps.shape) != shape[:-1] or exps.dtype != torch.uint8 or not exps.is_contiguous():
+            raise MiError("HistCache: exps must be a contiguous uint8 tensor of shape %s" % (shape[:-1],))
+        _need_cuda(kv, exps)
+        if exps is not None and exps.device != kv.device:
+            raise MiError("HistCache: kv and exps lie on different devices")
+        self.kv, self.exps, self.dtype = kv, exps, dtype
+        self.n_pages, self.n_heads, _, self.page_size, self.dim = shape
+        self.c = _lib.HistCacheC(kv=kv.data_ptr(), exps=exps.data_ptr() if exps is not None else None,
+                                 n_pages=self.n_pages, n_heads=self.n_heads, page_size=self.page_size, dim=self.dim,
+                                 dtype=self._DTYPES[dtype])
+        self._ref = ctypes.byref(self.c)
+
+    def ref(self):
+        return self._ref
+
+
+def _hist_common(what, cache, page_table, lengths, offsets, err, *more):
+    """Checks what every history call takes; returns the number of sequences."""
+    _need_cuda(page_table, lengths, offsets, err, *more)
+    dev = cache.kv.device
+    for t in (page_table, lengths, offsets, err) + more:
+        if t is not None and t.device != dev:
+            raise MiError("%s: a tensor lies on %s, the cache on %s" % (what, t.device, dev))
+    if _RAW_DEVICE is not None and dev.index != _RAW_DEVICE():
+        raise MiError("%s: the cache lies on %s, which is not the current device" % (what, dev))
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1 or \
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise MiError("%s: page_table must be int32 [sequences, pages] with contiguous rows" % what)
+    n = page_table.shape[0]
+    if tuple(lengths.shape) != (n,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        raise MiError("%s: lengths must be contiguous int32 [%d]" % (what, n))
+    if offsets is not None and (tuple(offsets.shape) != (n + 1,) or offsets.dtype != torch.int64 or
+                                not offsets.is_contiguous()):
+        raise MiError("%s: offsets must be contiguous int64 [%d]" % (what, n + 1))
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
+        raise MiError("%s: err must be an int32 error word (new_error_word)" % what)
+    return n
+
+
+def _hist_rows(what, cache, x):
+    if x.dim() != 3 or x.shape[1] != cache.n_heads or x.shape[2] != cache.dim:
+        raise MiError("%s: rows must be [n, %d, %d], got %s" % (what, cache.n_heads, cache.dim, tuple(x.shape)))
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("%s: rows must be float32 or bfloat16, got %s" % (what, x.dtype))
+    if x.stride(2) != 1:
+        raise MiError("%s: the values of a row must be contiguous" % what)
+    # a dimension of one entry is never stepped over: its stride says nothing
+    return x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
+
+
+def _hist_rows_call(name, what, cache, k, v, page_table, lengths, offsets, err):
+    n = _hist_common(what, cache, page_table, lengths, offsets, err, k, v)
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise MiError("%s: k and v differ in shape or type" % what)
+    (k_row, k_head), (v_row, v_head) = _hist_rows(what, cache, k), _hist_rows(what, cache, v)
+    if offsets is None and n and k.shape[0] % n:
+        raise MiError("%s: %d rows do not divide among %d sequences (pass offsets)" % (what, k.shape[0], n))
+    _lib.call(name, cache.ref(), _p(k), _p(v), MI_DT_BF16 if k.dtype == torch.bfloat16 else MI_DT_F32, k_row, k_head, v_row,
+              v_head, k.shape[0], _p(offsets), n, _p(page_table), page_table.stride(0), page_table.shape[1], _p(lengths),
+              _p(err), _stream())
+
+
+def hist_write(cache, k, v, page_table, lengths, offsets=None, err=None):
+    """Append rows k, v [n, heads, dim] (float32 or bfloat16, any row and head strides) to the sequences' pages, one launch.
+    Sequence b's rows - offsets[b] .. offsets[b+1], or n / sequences of them each - are its newest positions: ``lengths``
+    [sequences] int32 counts them already.  ``page_table`` [sequences, pages] int32.  Rows that no sequence owns, or
+    that would lie in front of position 0, are ignored; bad page ids and lengths beyond the table raise
+    MI_IDERR_RANGE in ``err``."""
+    _hist_rows_call('mi_hist_write', 'hist_write', cache, k, v, page_table, lengths, offsets, err)
+
+
+def hist_read(cache, page_table, lengths, n_rows=None, offsets=None, dtype=torch.bfloat16, out=None, err=None):
+    """The sequences' newest positions as packed rows (k, v) [n_rows, heads, dim], by hist_write's rule.  ``out`` = (k, v)
+    receives them when given (rows that no sequence owns stay as they are there; they are unset otherwise)."""
+    if out is None:
+        if n_rows is None:
+            raise MiError("hist_read: give n_rows or out")
+        shape = (int(n_rows), cache.n_heads, cache.dim)
+        out = (torch.empty(shape, dtype=dtype, device=cache.kv.device), torch.empty(shape, dtype=dtype, device=cache.kv.device))
+    elif n_rows is not None and out[0].shape[0] != n_rows:
+        raise MiError("hist_read: out holds %d rows, n_rows says %d" % (out[0].shape[0], n_rows))
+    k, v = out
+    _hist_rows_call('mi_hist_read', 'hist_read', cache, k, v, page_table, lengths, offsets, err)
+    return k, v
+
+
+def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
+    """Softmax attention of every sequence's new tokens or candidates ``q`` [sequences, heads, dim] or [sequences, tokens,
+    heads, dim] over all ``lengths`` positions of its history; the query heads share the cache's heads in equal groups.
+    q: float32 over a float32 cache, bfloat16 otherwise; the result has its shape and type.  ``scale``: of the scores,
+    dim ** -0.5 by default.  A sequence without history gives zeros."""
+    n = _hist_common('hist_attn', cache, page_table, lengths, None, err, q, out)
+    q4 = q.unsqueeze(1) if q.dim() == 3 else q
+    if q4.dim() != 4 or q4.shape[0] != n or q4.shape[3] != cache.dim or q4.shape[2] < 1 or q4.shape[2] % cache.n_heads:
+        raise MiError("hist_attn: q must be [%d, (tokens,) a multiple of %d heads, %d], got %s"
+                      % (n, cache.n_heads, cache.dim, tuple(q.shape)))
+    want = torch.float32 if cache.dtype == torch.float32 else torch.bfloat16
+    if q.dtype != want:
+        raise TypeError("hist_attn: q must be %s over a %s cache, got %s" % (want, cache.dtype, q.dtype))
+    if out is None:
+        out = torch.empty(q.shape, dtype=want, device=q.device)
+    elif out.shape != q.shape or out.dtype != want:
+        raise MiError("hist_attn: out must have q's shape and type")
+    o4 = out.unsqueeze(1) if out.dim() == 3 else out
+    if q4.stride(3) != 1 or o4.stride(3) != 1:
+        raise MiError("hist_attn: the values of a row must be contiguous")
+    qs, os_ = ([t.stride(d) if t.shape[d] > 1 else 0 for d in range(3)] for t in (q4, o4))
+    ws_bytes = _lib.load().mi_hist_attn_workspace_bytes(cache.ref(), n, q4.shape[1], q4.shape[2], page_table.shape[1])
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _lib.call('mi_hist_attn', cache.ref(), _p(q), qs[0], qs[1], qs[2], q4.shape[2], q4.shape[1], n, _p(page_table),
+              page_table.stride(0), page_table.shape[1], _p(lengths), cache.dim ** -0.5 if scale is None else scale, _p(out),
+              os_[0], os_[1], os_[2], _p(ws), ws_bytes, _p(err), _stream())
+    return out

@@ -1,0 +1,140 @@
+"""History cache without a GPU: the oracle's rules against hand-worked values, and every refusal of the entry points
+(the C ABI checks its arguments on the host before it touches the device)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import hist as oh
+
+
+def test_oracle_8_bit_rows_by_hand():
+    # 448 is the largest code: a row with maximum 448 keeps exponent 0, one step more moves to exponent 1
+    v, e = oh.quantise(np.array([[448.0, 1.0, 17.0, 0.0], [448.5, 1.0, -17.0, 18.0]]))
+    assert e.tolist() == [0, 1]
+    assert v[0].tolist() == [448.0, 1.0, 16.0, 0.0]             # 17 lies between 16 and 18: the even one
+    assert v[1].tolist() == [448.0, 1.0, -16.0, 18.0]           # 448.5 / 2 -> 224; 8.5 is a tie -> 8; 9 is a code
+    # maximum just above a power of two: exponent floor(log2) - 8
+    v, e = oh.quantise(np.array([[1.0, 2.0 ** -14, 2.0 ** -18, 0.0]]))
+    assert e.tolist() == [-8] and v[0].tolist() == [1.0, 2.0 ** -14, 0.0, 0.0]   # 2^-18 * 2^8 = half of 2^-9: to 0
+    # infinities and NaN do not set the exponent and come back as NaN
+    v, e = oh.quantise(np.array([[np.inf, 2.0, -np.inf, np.nan]]))
+    assert e.tolist() == [-7] and np.isnan(v[0]).tolist() == [True, False, True, True] and v[0, 1] == 2.0
+    v, e = oh.quantise(np.zeros((1, 4)))
+    assert e.tolist() == [-126] and not v.any()
+    # every e4m3 value is its own rounding (torch's codes as the independent table)
+    codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    codes = codes[np.isfinite(codes)]
+    assert np.array_equal(oh.e4m3_round(codes), codes) and codes.max() == oh.E4M3_MAX
+
+
+def test_oracle_rounding_equals_torchs_cast():
+    rng = np.random.default_rng(3)
+    x = (rng.standard_normal(200000) * np.exp2(rng.uniform(-12, 6, 200000))).astype(np.float32)
+    x = x[np.abs(x) <= 448]
+    want = torch.from_numpy(x).to(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(oh.e4m3_round(x), want)
+
+
+def test_oracle_places():
+    table = np.array([[4, 0, -1], [2, 9, 1]])
+    # 5 pages of 16: sequence 0 owns rows 0..2 as its positions 15, 16, 17; sequence 1 row 3 as position 40, in page 1
+    where, bad = oh.places(5, [0, 3, 4], 2, table, 16, 5, [18, 41])
+    assert where == [(4, 15), (0, 0), (0, 1), (1, 8), 'none'] and not bad
+    where, bad = oh.places(4, None, 2, table, 16, 5, [1, 20])    # position -1: no place; positions 18, 19 on page 9: bad
+    assert where == [None, (4, 0), None, None] and bad
+
+
+def test_oracle_attention_of_one_position_is_its_value():
+    rng = np.random.default_rng(0)
+    kv = rng.standard_normal((3, 2, 2, 16, 32))
+    q = rng.standard_normal((2, 1, 4, 32))
+    out, _, _ = oh.attention(kv, q, np.array([[2], [0]]), [1, 0], 0.1, 16)
+    for h in range(4):
+        np.testing.assert_allclose(out[0, 0, h], kv[2, h // 2, 1, 0], rtol=0, atol=0)
+    assert not out[1].any()
+
+
+# ------------------------------------------------------------------------------------------------ refusals (C ABI)
+def _cache(**over):
+    from recommendation_amd import _lib
+    args = dict(kv=4096, exps=None, n_pages=8, n_heads=2, page_size=16, dim=64, dtype=_lib.MI_DT_BF16)
+    args.update(over)
+    return _lib.HistCacheC(**args)
+
+
+@pytest.mark.parametrize('over, text', [
+    (dict(kv=None), 'null cache'), (dict(kv=4104), 'aligned'), (dict(dtype=3), 'dtype'), (dict(dim=48), 'dim'), (dict(dim=16), 'dim'),
+    (dict(dim=512), 'dim'), (dict(page_size=8), 'page_size'), (dict(page_size=48), 'page_size'),
+    (dict(page_size=2048), 'page_size'), (dict(n_heads=0), 'n_heads'), (dict(n_pages=0), 'n_pages'),
+    (dict(n_pages=1 << 31), 'n_pages'), (dict(exps=4096), 'exps'), (dict(dtype=2), 'exps'),
+])
+def test_bad_caches_are_refused(over, text):
+    from recommendation_amd import _lib
+    lib = _lib.load()
+    c = _cache(**over)
+    calls = [
+        lambda: lib.mi_hist_write(ctypes.byref(c), 4096, 4096, 1, 128, 64, 128, 64, 4, None, 4, 4096, 2, 2, 4096, None, None),
+        lambda: lib.mi_hist_read(ctypes.byref(c), 4096, 4096, 1, 128, 64, 128, 64, 4, None, 4, 4096, 2, 2, 4096, None, None),
+        lambda: lib.mi_hist_attn(ctypes.byref(c), 4096, 128, 128, 64, 2, 1, 4, 4096, 2, 2, 4096, 0.1, 4096, 128, 128, 64, None,
+                                 0, None, None)]
+    for call in calls:
+        assert call() == -1 and text in lib.mi_last_error().decode(), lib.mi_last_error()
+
+
+def test_bad_row_calls_are_refused():
+    from recommendation_amd import _lib
+    lib = _lib.load()
+    c = _cache()
+
+    def rc(k=4096, v=4096, dtype=1, strides=(128, 64, 128, 64), n=4, offsets=None, seqs=4, table=4096, ld=2, width=2,
+           lengths=4096):
+        out = {lib.mi_hist_write(ctypes.byref(c), k, v, dtype, *strides, n, offsets, seqs, table, ld, width, lengths, None, None),
+               lib.mi_hist_read(ctypes.byref(c), k, v, dtype, *strides, n, offsets, seqs, table, ld, width, lengths, None, None)}
+        assert len(out) == 1
+        return out.pop(), lib.mi_last_error().decode()
+
+    for kw, text in [(dict(k=None), 'null rows'), (dict(v=None), 'null rows'), (dict(dtype=2), 'f32 or bf16'),
+                     (dict(k=4104), '16-byte'), (dict(strides=(128, 64, 132, 64)), '16-byte'),
+                     (dict(strides=(128, 4, 128, 64)), '16-byte'), (dict(n=-1), 'n_rows'), (dict(n=6), 'divide'),
+                     (dict(table=None), 'page table'), (dict(lengths=None), 'lengths'), (dict(width=0), 'width'),
+                     (dict(ld=1), 'width'), (dict(seqs=-1), 'n_seqs')]:
+        code, msg = rc(**kw)
+        assert code == -1 and text in msg, (kw, msg)
+    code, msg = rc(n=1 << 30, offsets=4096)                      # 2^32 rows of K and V
+    assert code == -4 and 'in one call' in msg
+    assert rc(n=0)[0] == 0 and rc(seqs=0)[0] == 0                # nothing to do: no launch, no error
+
+
+def test_bad_attention_calls_are_refused():
+    from recommendation_amd import _lib
+    lib = _lib.load()
+    c = _cache()
+
+    def rc(q=4096, qs=(128, 128, 64), heads=2, tokens=1, seqs=4, table=4096, ld=2, width=2, lengths=4096, out=4096,
+           os_=(128, 128, 64)):
+        code = lib.mi_hist_attn(ctypes.byref(c), q, *qs, heads, tokens, seqs, table, ld, width, lengths, 0.1, out, *os_, None, 0,
+                                None, None)
+        return code, lib.mi_last_error().decode()
+
+    for kw, text in [(dict(q=None), 'null q'), (dict(out=None), 'null q or out'), (dict(heads=3), '3 heads'),
+                     (dict(heads=0), '0 heads'), (dict(tokens=-1), 'queries'), (dict(qs=(128, 128, 60)), '16-byte'),
+                     (dict(out=4100), '16-byte'), (dict(table=None), 'page table'), (dict(width=0), 'width'),
+                     (dict(lengths=None), 'lengths'), (dict(tokens=70000), 'query rows')]:
+        code, msg = rc(**kw)
+        assert code == -1 and text in msg, (kw, msg)
+    assert rc(tokens=0)[0] == 0 and rc(seqs=0)[0] == 0
+
+
+def test_host_tensors_are_refused():
+    from recommendation_amd import ops
+    with pytest.raises(ops.MiError, match='device tensors'):
+        ops.HistCache(4, 16, 2, 64, device='cpu')
+    for bad in (dict(page_size=8), dict(page_size=24), dict(dim=48), dict(n_pages=0)):
+        args = dict(n_pages=4, page_size=16, n_heads=2, dim=64)
+        args.update(bad)
+        with pytest.raises(ops.MiError, match='HistCache'):
+            ops.HistCache(device='cpu', **args)
+    with pytest.raises(TypeError, match='HistCache'):
+        ops.HistCache(4, 16, 2, 64, dtype=torch.float16, device='cpu')

@@ -1,0 +1,497 @@
+"""History cache on the GPU: hist_write / hist_read bit for bit and hist_attn within derived bounds of oracle/hist.py.
+
+Bounds of the attention, per output element, with P|v| = sum_j p_j |v_jd| and u = 2^-24 (half an f32 step):
+  scores     a dot product of `dim` exact or f32 products accumulated in f32, scaled twice: off by at most
+             (dim + 4) u A, A = max_j sum_d |q_d k_jd| * scale; the weights exp(s_j - m) then by
+             ds = 2 (dim + 4) u A + 8 u (max subtracted, exponential), numerator and denominator: 2 ds P|v|
+  sums       n terms in f32, numerator and denominator: 2 (n + 16) u P|v|
+  8, 16 bit  weights rounded to bf16, delta <= 2^-8 each, divided by the sum of the ROUNDED weights:
+             o' - o = sum p delta (v - o) / sum p (1 + delta), at most 2^-8 (1 + 2^-7) (P|v| + |o|);
+             the output rounded to bf16: 2^-8 of itself
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import hist as oh
+from tests.errlog import held
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {'f32': torch.float32, 'bf16': torch.bfloat16, 'e4m3': torch.float8_e4m3fn}
+U = 2.0 ** -24
+
+
+def bound(cache, dim, n, want, absv, size):
+    ds = 2 * (dim + 4) * U * size[..., None] + 8 * U
+    b = (2 * ds + 2 * (n + 16) * U) * absv
+    if cache != 'f32':
+        b = b + 2.0 ** -8 * (1 + 2.0 ** -7) * (absv + np.abs(want))
+        b = b + 2.0 ** -8 * (np.abs(want) + b)
+    return b + 1e-37
+
+
+def poisoned(dev, cache, n_pages, page, heads, dim):
+    """A cache whose every byte is a NaN."""
+    from recommendation_amd import ops
+    c = ops.HistCache(n_pages, page, heads, dim, dtype=DTYPES[cache], device=dev)
+    if cache == 'e4m3':
+        c.kv.view(torch.uint8).fill_(0x7f)
+        c.exps.fill_(255)
+    else:
+        c.kv.fill_(float('nan'))
+    return c
+
+
+def values(c):
+    """The cache as the float64 values it stands for."""
+    if c.exps is None:
+        return c.kv.double().cpu().numpy()
+    return np.ldexp(c.kv.cpu().double().numpy(), c.exps.cpu().numpy().astype(np.int64)[..., None] - 127)
+
+
+def tables(rng, lens, page, width, n_pages):
+    """A shuffled page table with -1 behind every history; distinct pages."""
+    t = np.full((len(lens), width), -1, np.int32)
+    order = rng.permutation(n_pages)
+    at = 0
+    for b, n in enumerate(lens):
+        k = -(-max(n, 0) // page)
+        t[b, :k] = order[at:at + k]
+        at += k
+    assert at <= n_pages
+    return t
+
+
+def filled(dev, rng, cache, lens, page, heads, dim, spare=3, given=torch.float32, width=None, scale_rows=True):
+    """A cache with random histories written through hist_write; everything else in it is NaN."""
+    from recommendation_amd import ops
+    need = sum(-(-max(n, 0) // page) for n in lens)
+    width = width or max(1, max(-(-max(n, 0) // page) for n in lens)) + 1
+    c = poisoned(dev, cache, need + spare, page, heads, dim)
+    t = tables(rng, lens, page, width, need + spare)
+    own = [max(n, 0) for n in lens]
+    offs = np.concatenate([[0], np.cumsum(own)]).astype(np.int64)
+    k = rng.standard_normal((int(offs[-1]), heads, dim))
+    v = rng.standard_normal((int(offs[-1]), heads, dim))
+    if scale_rows:
+        v *= np.exp2(rng.integers(-3, 4, size=(int(offs[-1]), heads, 1)))
+    table, lengths = torch.from_numpy(t).to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+    if offs[-1]:
+        ops.hist_write(c, torch.from_numpy(k).to(dev, given), torch.from_numpy(v).to(dev, given), table, lengths,
+                       offsets=torch.from_numpy(offs).to(dev))
+    return c, table, lengths, t
+
+
+# ------------------------------------------------------------------------------------------------ write and read
+@pytest.mark.parametrize('given', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('dim, heads, page', [(32, 1, 16), (64, 3, 16), (128, 2, 64), (256, 5, 32)])
+def test_write_and_read_are_exact(dev, cache, given, dim, heads, page):
+    from recommendation_amd import ops
+    rng = np.random.default_rng(dim + heads)
+    lens = [0, 1, 15, 16, 17, 40, 3, 100, 33, 5]
+    new = [0, 1, 15, 7, 17, 0, 3, 64, 1, 2]
+    width = 8
+    n_pages = 40
+    t = tables(rng, lens, page, width, n_pages)
+    offs = np.concatenate([[0], np.cumsum(new)]).astype(np.int64)
+    n = int(offs[-1]) + 4                                                    # four rows behind the last sequence
+    x = rng.standard_normal((n, 2, heads, dim)) * np.exp2(rng.integers(-30, 30, size=(n, 2, heads, 1)))
+    x[3] = 0.0
+    x[4, :, 0, 0], x[5, 1, 0, 1] = np.inf, -np.inf
+    x[6, 0, heads - 1, 2] = np.nan
+    x[7] *= 1e-38 / np.abs(x[7]).max()                                       # exponents at the bottom
+    rows = torch.from_numpy(x).to(dev, given)
+    k, v = rows[:, 0], rows[:, 1]                                            # strided: K and V side by side
+    c = poisoned(dev, cache, n_pages, page, heads, dim)
+    want = values(c)
+    err = ops.new_error_word(dev)
+    table, lengths, offsets = torch.from_numpy(t).to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), \
+        torch.from_numpy(offs).to(dev)
+    ops.hist_write(c, k, v, table, lengths, offsets=offsets, err=err)
+    where, bad = oh.places(n, offs, len(lens), t, page, n_pages, lens)
+    assert not bad and err.item() == 0
+    held_rows = rows.double().cpu().numpy()
+    if cache == 'e4m3':
+        held_rows, exponents = oh.quantise(held_rows)
+        for i, w in enumerate(where):
+            if isinstance(w, tuple):
+                got = c.exps[w[0], :, :, w[1]].cpu().numpy().astype(np.int64) - 127
+                assert np.array_equal(got, exponents[i].T)
+    elif cache == 'bf16':
+        held_rows = torch.from_numpy(held_rows).to(torch.bfloat16).double().numpy()
+    oh.write(want, held_rows[:, 0], held_rows[:, 1], where)
+    np.testing.assert_array_equal(values(c), want)                           # every other byte is still a NaN
+    for dtype in (torch.float32, torch.bfloat16):
+        out = tuple(torch.full((n, heads, dim), 7.0, dtype=dtype, device=dev) for _ in range(2))
+        ops.hist_read(c, table, lengths, offsets=offsets, out=out, err=err)
+        wk, wv = np.full((n, heads, dim), 7.0), np.full((n, heads, dim), 7.0)
+        oh.read(want, where, wk, wv)
+        for got, w in ((out[0], wk), (out[1], wv)):
+            w = torch.from_numpy(w).to(torch.float32).to(dtype)
+            np.testing.assert_array_equal(got.float().cpu().numpy(), w.float().numpy())
+    assert err.item() == 0
+
+
+def test_rows_without_a_place(dev):
+    """Lengths shorter than the rows given, padded sequences, bad pages and histories beyond the table."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(1)
+    page, heads, dim, n_pages = 16, 2, 64, 10
+    lens = [2, 0, 20, 36, -5, 40]
+    t = np.array([[3, -1], [0, 0], [7, 10], [1, 2], [4, 4], [5, -3]], np.int32)
+    offs = np.array([0, 4, 6, 12, 18, 20, 30], np.int64)
+    x = rng.standard_normal((30, 2, heads, dim))
+    rows = torch.from_numpy(x).to(dev, torch.bfloat16)
+    table, lengths = torch.from_numpy(t).to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+    where, bad = oh.places(30, offs, 6, t, page, n_pages, lens)
+    assert bad and None in where
+    for cache in ('bf16', 'e4m3'):
+        c, err = poisoned(dev, cache, n_pages, page, heads, dim), ops.new_error_word(dev)
+        want = values(c)
+        held_rows = rows.double().cpu().numpy()
+        if cache == 'e4m3':
+            held_rows = oh.quantise(held_rows)[0]
+        oh.write(want, held_rows[:, 0], held_rows[:, 1], where)
+        ops.hist_write(c, rows[:, 0], rows[:, 1], table, lengths, offsets=torch.from_numpy(offs).to(dev), err=err)
+        np.testing.assert_array_equal(values(c), want)
+        with pytest.raises(ops.InvalidArgumentError, match='out of bounds'):
+            ops.check_error_word(err, 'pages')
+        k, v = ops.hist_read(c, table, lengths, 30, offsets=torch.from_numpy(offs).to(dev), dtype=torch.float32, err=err)
+        wk, wv = np.zeros((30, heads, dim)), np.zeros((30, heads, dim))
+        oh.read(want, where, wk, wv)
+        np.testing.assert_array_equal(k.cpu().numpy(), wk.astype(np.float32))
+        np.testing.assert_array_equal(v.cpu().numpy(), wv.astype(np.float32))
+        assert err.item() == 1
+    # without an error word the same call just skips
+    ops.hist_write(c, rows[:, 0], rows[:, 1], table, lengths, offsets=torch.from_numpy(offs).to(dev))
+    # padded sequences alone are no error
+    err = ops.new_error_word(dev)
+    ops.hist_write(c, rows[:2, 0], rows[:2, 1], table[1:3], torch.tensor([0, 1], dtype=torch.int32, device=dev), err=err)
+    assert err.item() == 0
+
+
+@pytest.mark.parametrize('users', [1, 63, 64, 65, 700, 5000])
+def test_offsets_of_many_sequences(dev, users):
+    """Every search depth: empty sequences, runs of them at both ends, and one event each without offsets."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(users)
+    page, heads, dim = 16, 1, 32
+    new = rng.integers(0, 4, size=users)
+    new[:users // 3] = 0
+    new[-(users // 5):] = 0
+    if users == 1:
+        new[:] = 3
+    lens = (new + rng.integers(0, 10, size=users)).astype(np.int32)
+    t = tables(rng, lens, page, 1, users + 2)
+    offs = np.concatenate([[0], np.cumsum(new)]).astype(np.int64)
+    n = int(offs[-1])
+    x = torch.from_numpy(rng.standard_normal((n, 2, heads, dim))).to(dev, torch.float32)
+    c = poisoned(dev, 'f32', users + 2, page, heads, dim)
+    want = values(c)
+    table, lengths = torch.from_numpy(t).to(dev), torch.from_numpy(lens).to(dev)
+    ops.hist_write(c, x[:, 0], x[:, 1], table, lengths, offsets=torch.from_numpy(offs).to(dev))
+    where, bad = oh.places(n, offs, users, t, page, users + 2, lens)
+    assert not bad
+    oh.write(want, x[:, 0].double().cpu().numpy(), x[:, 1].double().cpu().numpy(), where)
+    np.testing.assert_array_equal(values(c), want)
+    one = torch.from_numpy(rng.standard_normal((users, 2, heads, dim))).to(dev, torch.float32)
+    lengths = (lengths + 1).to(torch.int32).clamp(max=16)
+    live = t[:, 0] >= 0
+    ops.hist_write(c, one[:, 0], one[:, 1], table, lengths)
+    k, v = ops.hist_read(c, table, lengths, users, dtype=torch.float32)
+    np.testing.assert_array_equal(k.cpu().numpy()[live], one[:, 0].cpu().numpy()[live])
+    np.testing.assert_array_equal(v.cpu().numpy()[live], one[:, 1].cpu().numpy()[live])
+    assert not k.cpu().numpy()[~live].any()
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def run_attn(dev, rng, cache, lens, page, heads, group, tokens, dim, width=None, name='', scale=None, queries=None):
+    from recommendation_amd import ops
+    c, table, lengths, t = filled(dev, rng, cache, lens, page, heads, dim, width=width)
+    dt = torch.float32 if cache == 'f32' else torch.bfloat16
+    n, Hq = len(lens), heads * group
+    q = rng.standard_normal((n, tokens, Hq, dim)) * 1.5 if queries is None else queries
+    q = torch.from_numpy(q).to(dev, dt)
+    out = torch.full((n, tokens, Hq, dim + 16), 3.0, dtype=dt, device=dev)   # rows with a gap behind them
+    err = ops.new_error_word(dev)
+    got = ops.hist_attn(c, q, table, lengths, scale=scale, out=out[..., :dim], err=err)
+    assert got.data_ptr() == out.data_ptr() and err.item() == 0
+    assert bool((out[..., dim:] == 3.0).all())
+    s = dim ** -0.5 if scale is None else scale
+    want, absv, size = oh.attention(values(c), q.double().cpu().numpy(), t, lens, s, page)
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    b = bound(cache, dim, max(max(lens), 1), want, absv, size)
+    held("hist_attn %s dim %d page %d heads %dx%d tokens %d %s" % (cache, dim, page, heads, group, tokens, name),
+         (np.abs(got - want) / b).max(), 1.0)
+    for i, x in enumerate(lens):
+        if x <= 0:
+            assert not got[i].any()
+    return c, table, lengths, q, out
+
+
+EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 63, 64, 65, 100, 127, 128, 129, 200, 0]
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('dim', [32, 64, 128, 256])
+def test_attention_at_every_edge_of_tile_and_page(dev, cache, dim):
+    rng = np.random.default_rng(dim)
+    for page, heads, group, tokens in ((16, 1, 1, 1), (64, 2, 4, 1), (32, 3, 5, 2), (128, 1, 7, 5)):
+        run_attn(dev, rng, cache, EDGES, page, heads, group, tokens, dim)
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('lens, heads, group, tokens, dim, page', [
+    ([5000], 1, 1, 1, 64, 16), ([1023, 1, 0, 4097], 2, 8, 1, 128, 64), ([3000, 10, 2999], 1, 16, 1, 64, 1024),
+    ([2500, 700], 2, 3, 11, 32, 32), ([1500, 1], 1, 1, 70, 256, 16), ([900] * 40, 4, 2, 1, 64, 16)])
+def test_attention_over_long_histories(dev, cache, lens, heads, group, tokens, dim, page):
+    run_attn(dev, np.random.default_rng(len(lens) + dim), cache, lens, page, heads, group, tokens, dim)
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_attention_of_many_short_histories(dev, cache):
+    """The DIN shape: thousands of samples with up to 100 events, one head."""
+    rng = np.random.default_rng(9)
+    lens = rng.integers(0, 101, size=1500).tolist()
+    run_attn(dev, rng, cache, lens, 16, 1, 1, 1, 64, width=7)
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_attention_with_peaked_and_flat_scores(dev, cache):
+    """One position takes all the weight, early or late; and scale 0: the plain mean."""
+    rng = np.random.default_rng(4)
+    lens = [300, 77, 1]
+    run_attn(dev, rng, cache, lens, 16, 2, 2, 1, 64, scale=4.0, name='peaked')
+    run_attn(dev, rng, cache, lens, 16, 2, 2, 1, 64, scale=0.0, name='mean')
+    run_attn(dev, rng, cache, lens, 16, 2, 2, 1, 64, scale=-0.3, name='negative scale')
+
+
+@pytest.mark.parametrize('cache', ['bf16', 'e4m3'])
+def test_strided_queries_shared_pages_and_table_views(dev, cache):
+    """Queries as a slice of a fused projection, several sequences on the same pages, a page table that is a view."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(12)
+    c, table, lengths, t = filled(dev, rng, cache, [200, 90], 32, 2, 64)
+    wide = torch.full((5, 20), -1, dtype=torch.int32, device=dev)
+    wide[:, 3:3 + table.shape[1]] = table[torch.tensor([0, 1, 0, 0, 1], device=dev)]
+    lens = [200, 90, 150, 1, 33]
+    lengths = torch.tensor(lens, dtype=torch.int32, device=dev)
+    fused = torch.from_numpy(rng.standard_normal((5, 3 * 8 * 64))).to(dev, torch.bfloat16)
+    q = fused[:, 512:1024].view(5, 8, 64)
+    view = wide[:, 3:3 + table.shape[1]]
+    got = ops.hist_attn(c, q, view, lengths)
+    assert got.shape == (5, 8, 64)
+    want, absv, size = oh.attention(values(c), q.double().cpu().numpy()[:, None], view.cpu().numpy(), lens, 64 ** -0.5, 32)
+    b = bound(cache, 64, 200, want, absv, size)
+    held("hist_attn %s strided" % cache, (np.abs(got.double().cpu().numpy()[:, None] - want) / b).max(), 1.0)
+    # heads transposed: tokens and heads of a [heads, tokens] tensor
+    qt = torch.from_numpy(rng.standard_normal((5, 4, 3, 64))).to(dev, torch.bfloat16).transpose(1, 2)
+    got = ops.hist_attn(c, qt, view, lengths)
+    want, absv, size = oh.attention(values(c), qt.double().cpu().numpy(), view.cpu().numpy(), lens, 64 ** -0.5, 32)
+    held("hist_attn %s transposed" % cache, (np.abs(got.double().cpu().numpy() - want) / bound(cache, 64, 200, want, absv, size)).max(), 1.0)
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_bad_pages_are_absent_and_reported(dev, cache):
+    from recommendation_amd import ops
+    rng = np.random.default_rng(21)
+    lens = [100, 1000, 64, 40]
+    c, table, lengths, t = filled(dev, rng, cache, lens, 16, 2, 64, width=63)
+    t = t.copy()
+    t[0, 2], t[0, 6], t[1, 5], t[1, 30:34] = -1, c.n_pages, 1 << 30, -7
+    t[3, :] = -1                                                             # no page at all: zeros
+    lens[2] = 64
+    dt = torch.float32 if cache == 'f32' else torch.bfloat16
+    q = torch.from_numpy(rng.standard_normal((4, 1, 4, 64))).to(dev, dt)
+    err = ops.new_error_word(dev)
+    got = ops.hist_attn(c, q, torch.from_numpy(t).to(dev), lengths, err=err).double().cpu().numpy()
+    want, absv, size = oh.attention(values(c), q.double().cpu().numpy(), t, lens, 64 ** -0.5, 16)
+    held("hist_attn %s bad pages" % cache, (np.abs(got - want) / bound(cache, 64, 1000, want, absv, size)).max(), 1.0)
+    assert not got[3].any() and err.item() == 1
+    # a length beyond the table: its pages' positions only, reported
+    err = ops.new_error_word(dev)
+    got2 = ops.hist_attn(c, q[2:3], table[2:3, :4], torch.tensor([70], dtype=torch.int32, device=dev), err=err)
+    assert err.item() == 1
+    np.testing.assert_array_equal(got2.double().cpu().numpy()[0], got[2])
+    ops.hist_attn(c, q[2:3], table[2:3, :4], torch.tensor([64], dtype=torch.int32, device=dev), err=ops.new_error_word(dev))
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16'])
+def test_infinite_and_nan_values(dev, cache):
+    """Rows without a finite score give zeros; an infinite score or a NaN in a live position shows as NaN."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(31)
+    dt = DTYPES[cache]
+    c, table, lengths, t = filled(dev, rng, cache, [40, 40, 40, 40], 16, 1, 64)
+    q = torch.from_numpy(rng.standard_normal((4, 1, 1, 64))).to(dev, dt)
+    q[:, 0, 0, 0] = 1.0
+    clean = ops.hist_attn(c, q, table, lengths)
+    page = t[0]
+    c.kv[page[:3].tolist(), 0, 0, :, 0] = -float('inf')                      # sequence 0: every score -inf
+    c.kv[int(t[1][1]), 0, 0, 5, 0] = -float('inf')                           # sequence 1: one position drops out
+    c.kv[int(t[2][2]), 0, 0, 2, 3] = float('nan')                            # sequence 2: a NaN key in a live position
+    got = ops.hist_attn(c, q, table, lengths)
+    assert not got[0].any()
+    assert torch.isnan(got[2]).all()
+    assert torch.equal(got[3], clean[3])
+    want, absv, size = oh.attention(values(c)[:, :, :, :, :], q.double().cpu().numpy(), t, [0, 40, 0, 0], 0.125, 16)
+    size = np.where(np.isfinite(size), size, 64.0)
+    err = (np.abs(got[1].double().cpu().numpy() - want[1]) / bound(cache, 64, 40, want, absv, size)[1]).max()
+    held("hist_attn %s one -inf score" % cache, err, 1.0)
+
+
+# ------------------------------------------------------------------------------------------------ used together
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_histories_grow_event_by_event(dev, cache):
+    """The serving loop: prompts in one call, then one event a step for a batch in which some users pause (length 0),
+    attention after each; captured once and replayed on new inputs, equal to the eager calls bit for bit."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(5)
+    dt = torch.float32 if cache == 'f32' else torch.bfloat16
+    heads, group, dim, page, users, width = 2, 3, 64, 16, 6, 6
+    c = poisoned(dev, cache, users * width, page, heads, dim)
+    twin = poisoned(dev, cache, users * width, page, heads, dim)
+    table = torch.from_numpy(rng.permutation(users * width).astype(np.int32).reshape(users, width)).to(dev)
+    start = np.array([0, 14, 15, 16, 31, 50])
+    offs = np.concatenate([[0], np.cumsum(start)]).astype(np.int64)
+    rows = torch.from_numpy(rng.standard_normal((int(offs[-1]), 2, heads, dim))).to(dev, dt)
+    lens = torch.from_numpy(start.astype(np.int32)).to(dev)
+    for x in (c, twin):
+        ops.hist_write(x, rows[:, 0], rows[:, 1], table, lens, offsets=torch.from_numpy(offs).to(dev))
+    k, v = (torch.zeros((users, heads, dim), dtype=dt, device=dev) for _ in range(2))
+    q = torch.zeros((users, heads * group, dim), dtype=dt, device=dev)
+    step_lens = lens.clone()
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                                            # a length of 0 pauses everybody: no effect
+        zero = torch.zeros_like(lens)
+        ops.hist_write(c, k, v, table, zero)
+        ops.hist_attn(c, q, table, zero, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    assert not out.any()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.hist_write(c, k, v, table, step_lens)
+        ops.hist_attn(c, q, table, step_lens, out=out)
+    held_len = start.copy()
+    for step in range(20):
+        k.copy_(torch.from_numpy(rng.standard_normal(tuple(k.shape))))
+        v.copy_(torch.from_numpy(rng.standard_normal(tuple(k.shape))))
+        q.copy_(torch.from_numpy(rng.standard_normal(tuple(q.shape))))
+        paused = rng.random(users) < 0.3
+        held_len = held_len + ~paused
+        now = np.where(paused, 0, held_len).astype(np.int32)
+        step_lens.copy_(torch.from_numpy(now))
+        graph.replay()
+        ops.hist_write(twin, k, v, table, step_lens)
+        eager = ops.hist_attn(twin, q, table, step_lens)
+        assert torch.equal(out, eager)
+        assert not out[torch.from_numpy(paused).to(dev)].any()
+    np.testing.assert_array_equal(values(c), values(twin))
+    final = torch.from_numpy(held_len.astype(np.int32)).to(dev)
+    got = ops.hist_attn(c, q, table, final).double().cpu().numpy()[:, None]
+    want, absv, size = oh.attention(values(c), q.double().cpu().numpy()[:, None], table.cpu().numpy(), held_len, dim ** -0.5, page)
+    held("hist_attn %s grown" % cache, (np.abs(got - want) / bound(cache, dim, 80, want, absv, size)).max(), 1.0)
+    # the histories read back and written into a fresh cache are the same histories
+    total = int(held_len.sum())
+    offs = torch.from_numpy(np.concatenate([[0], np.cumsum(held_len)]).astype(np.int64)).to(dev)
+    k2, v2 = ops.hist_read(c, table, final, total, offsets=offs, dtype=torch.float32)
+    fresh = poisoned(dev, cache, users * width, page, heads, dim)
+    ops.hist_write(fresh, k2, v2, table, final, offsets=offs)
+    np.testing.assert_array_equal(values(fresh), values(c))
+
+
+def test_two_calls_at_once_on_two_streams(dev):
+    """Calls that share nothing but the cache they read run side by side with their own workspaces."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(6)
+    c, table, lengths, t = filled(dev, rng, 'bf16', [9000, 100, 4000], 16, 2, 64)
+    qs = [torch.from_numpy(rng.standard_normal((3, 8, 64))).to(dev, torch.bfloat16) for _ in range(2)]
+    want = [ops.hist_attn(c, q, table, lengths) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.hist_attn(c, qs[i], table, lengths))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_offsets_into_a_pool_past_32_bits(dev):
+    """Pages whose bytes, and element indexes, lie past 2^32."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(8)
+    page, heads, dim = 1024, 8, 256
+    n_pages = (1 << 33) // (heads * 2 * page * dim) + 5                       # 2^33 elements of 8 bits
+    kv = torch.empty((n_pages, heads, 2, page, dim), dtype=torch.uint8, device=dev)
+    kv[-4:].fill_(0x7f)
+    c = ops.HistCache(n_pages, page, heads, dim, dtype=torch.float8_e4m3fn, kv=kv.view(torch.float8_e4m3fn))
+    table = torch.tensor([[n_pages - 1, n_pages - 3], [n_pages - 2, -1]], dtype=torch.int32, device=dev)
+    lens = [1100, 3]
+    lengths = torch.tensor(lens, dtype=torch.int32, device=dev)
+    offs = torch.tensor([0, 1100, 1103], dtype=torch.int64, device=dev)
+    rows = torch.from_numpy(rng.standard_normal((1103, 2, heads, dim))).to(dev, torch.bfloat16)
+    ops.hist_write(c, rows[:, 0], rows[:, 1], table, lengths, offsets=offs)
+    k, v = ops.hist_read(c, table, lengths, 1103, offsets=offs, dtype=torch.float32)
+    held_rows = oh.quantise(rows.double().cpu().numpy())[0]
+    np.testing.assert_array_equal(k.cpu().numpy(), held_rows[:, 0].astype(np.float32))
+    np.testing.assert_array_equal(v.cpu().numpy(), held_rows[:, 1].astype(np.float32))
+    q = torch.from_numpy(rng.standard_normal((2, 1, heads, dim))).to(dev, torch.bfloat16)
+    got = ops.hist_attn(c, q, table, lengths).double().cpu().numpy()
+    small = np.zeros((3, heads, 2, page, dim))
+    small[0, :, 0], small[0, :, 1] = held_rows[:1024, 0].transpose(1, 0, 2), held_rows[:1024, 1].transpose(1, 0, 2)
+    small[1, :, 0, :76], small[1, :, 1, :76] = held_rows[1024:1100, 0].transpose(1, 0, 2), held_rows[1024:1100, 1].transpose(1, 0, 2)
+    small[2, :, 0, :3], small[2, :, 1, :3] = held_rows[1100:, 0].transpose(1, 0, 2), held_rows[1100:, 1].transpose(1, 0, 2)
+    want, absv, size = oh.attention(small, q.double().cpu().numpy(), np.array([[0, 1], [2, -1]]), lens, dim ** -0.5, page)
+    held("hist_attn past 2^32", (np.abs(got - want) / bound('e4m3', dim, 1100, want, absv, size)).max(), 1.0)
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_calls_that_do_not_fit_are_refused(dev):
+    from recommendation_amd import ops
+    c = ops.HistCache(8, 16, 2, 64, device=dev)
+    c.kv.zero_()
+    table = torch.zeros((3, 2), dtype=torch.int32, device=dev)
+    lengths = torch.zeros(3, dtype=torch.int32, device=dev)
+    k = torch.zeros((3, 2, 64), dtype=torch.bfloat16, device=dev)
+    q = torch.zeros((3, 4, 64), dtype=torch.bfloat16, device=dev)
+    for bad, exc, text in [
+            (lambda: ops.hist_write(c, k.half(), k.half(), table, lengths), TypeError, 'float32 or bfloat16'),
+            (lambda: ops.hist_write(c, k, k.float(), table, lengths), ops.MiError, 'differ'),
+            (lambda: ops.hist_write(c, k[:, :1], k[:, :1], table, lengths), ops.MiError, 'rows must be'),
+            (lambda: ops.hist_write(c, k[:2], k[:2], table, lengths), ops.MiError, 'divide'),
+            (lambda: ops.hist_write(c, k, k, table.long(), lengths), ops.MiError, 'page_table'),
+            (lambda: ops.hist_write(c, k, k, table.t(), lengths), ops.MiError, 'page_table'),
+            (lambda: ops.hist_write(c, k, k, table, lengths.long()), ops.MiError, 'lengths'),
+            (lambda: ops.hist_write(c, k, k, table, lengths[:2]), ops.MiError, 'lengths'),
+            (lambda: ops.hist_write(c, k, k, table, lengths, offsets=lengths), ops.MiError, 'offsets'),
+            (lambda: ops.hist_write(c, k.cpu(), k.cpu(), table, lengths), ops.MiError, 'device tensors'),
+            (lambda: ops.hist_write(c, k.transpose(1, 2).contiguous().transpose(1, 2), k, table, lengths), ops.MiError, 'contiguous'),
+            (lambda: ops.hist_write(c, torch.zeros(3 * 128 + 4, dtype=torch.bfloat16, device=dev)[4:].view(3, 2, 64), k, table, lengths),
+             ops.MiError, '16-byte'),
+            (lambda: ops.hist_read(c, table, lengths), ops.MiError, 'n_rows'),
+            (lambda: ops.hist_read(c, table, lengths, 3, dtype=torch.float16), TypeError, 'float32 or bfloat16'),
+            (lambda: ops.hist_read(c, table, lengths, 4, out=(k, k.clone())), ops.MiError, 'n_rows'),
+            (lambda: ops.hist_attn(c, q.float(), table, lengths), TypeError, 'bfloat16'),
+            (lambda: ops.hist_attn(c, q[:, :3], table, lengths), ops.MiError, 'multiple'),
+            (lambda: ops.hist_attn(c, q[:2], table, lengths), ops.MiError, 'q must be'),
+            (lambda: ops.hist_attn(c, q, table, lengths, out=q.float()), ops.MiError, 'out'),
+            (lambda: ops.hist_attn(c, q, table, lengths, err=torch.zeros(1, device=dev)), ops.MiError, 'err'),
+            (lambda: ops.HistCache(8, 16, 2, 64, kv=c.kv[:4]), ops.MiError, 'kv must be'),
+            (lambda: ops.HistCache(8, 16, 2, 64, kv=c.kv, exps=torch.zeros((8, 2, 2, 16), dtype=torch.uint8, device=dev)), ops.MiError, 'exps'),
+            (lambda: ops.HistCache(8, 16, 2, 64, dtype=torch.float8_e4m3fn, device=dev, kv=None,
+                                   exps=torch.zeros((8, 2, 2, 16), dtype=torch.uint8, device=dev)), ops.MiError, 'exps')]:
+        with pytest.raises(exc, match=text):
+            bad()
+    # nothing to do
+    ops.hist_write(c, k[:0], k[:0], table[:0], lengths[:0])
+    assert ops.hist_attn(c, q[:0], table[:0], lengths[:0]).shape == (0, 4, 64)
+    assert ops.hist_attn(c, q.view(3, 1, 4, 64)[:, :0], table, lengths).shape == (3, 0, 4, 64)
+    assert ops.hist_read(c, table, lengths, 0)[0].shape == (0, 2, 64)
