@@ -321,7 +321,7 @@ struct AttnArgs {
 // its right operand if its reduction index is read as "positions 4g..4g+3 of tile 0, then of tile 1".  Its left
 // operand takes output channels j of 16 lanes' 16-byte pieces of a V row, whatever those channels are called.  So no
 // score, probability or value crosses lanes; only the row maximum and sum do (over the four g).
-template <int DT, int D>
+template <int DT, int D, int RT>
 struct Wave {
   static constexpr bool F32 = DT == MI_DT_F32;
   static constexpr int E = Elem<DT>::BYTES;
@@ -337,10 +337,10 @@ struct Wave {
   static constexpr int CHUNK = 32;                          // positions per step, two tiles
   static constexpr int NS = D / 32;                         // 32-channel steps of the score product (8 / 16 bit)
 
-  f4v o[VH][VE];
-  float m, l;
-  bf8v qf[F32 ? 1 : NS];
-  f4v qv[F32 ? KL : 1];
+  f4v o[RT][VH][VE];
+  float m[RT], l[RT];
+  bf8v qf[RT][F32 ? 1 : NS];
+  f4v qv[RT][F32 ? KL : 1];
 
   // channel of element 0 of this lane's query fragment of step s
   static __device__ __forceinline__ int q_channel(int s, int g) {
@@ -348,24 +348,24 @@ struct Wave {
     return s * 32 + g * 8;
   }
 
-  __device__ __forceinline__ void init(const char* q_row, bool live, int g) {
-    m = -INFINITY;
-    l = 0.f;
+  __device__ __forceinline__ void init(int t, const char* q_row, bool live, int g) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
 #pragma unroll
     for (int h = 0; h < VH; ++h)
 #pragma unroll
-      for (int j = 0; j < VE; ++j) o[h][j] = f4v{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < VE; ++j) o[t][h][j] = f4v{0.f, 0.f, 0.f, 0.f};
     if constexpr (F32) {
 #pragma unroll
       for (int s = 0; s < KL; ++s) {
         const f4v x = *reinterpret_cast<const f4v*>(q_row + (s * 16 + g * 4) * 4);
-        qv[s] = live ? x : f4v{0.f, 0.f, 0.f, 0.f};
+        qv[t][s] = live ? x : f4v{0.f, 0.f, 0.f, 0.f};
       }
     } else {
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const uint4 x = *reinterpret_cast<const uint4*>(q_row + q_channel(s, g) * 2);
-        qf[s] = __builtin_bit_cast(bf8v, live ? x : make_uint4(0, 0, 0, 0));
+        qf[t][s] = __builtin_bit_cast(bf8v, live ? x : make_uint4(0, 0, 0, 0));
       }
     }
   }
@@ -374,6 +374,7 @@ struct Wave {
     unsigned int k[2][KL][KB / 4];
     unsigned int v[2][4][VH][VB < 4 ? 1 : VB / 4];
     unsigned int ek[2], ev[2];
+    int valid[2];                                           // live positions of each tile, the same in every lane
   };
 
   template <int BYTES>
@@ -391,9 +392,25 @@ struct Wave {
     }
   }
 
-  // rows: index of the tile's first K row in the cache (V lies page_size rows behind)
-  __device__ __forceinline__ void request(Fetched& f, const AttnArgs& p, const int64_t (&rows)[2], int g, int c) {
-    const int page = 1 << p.page_shift;
+  // Requests the 32 positions from `pos` of a history of `len` (table: the sequence's pages).  Tiles behind the end,
+  // or on a bad page, read page 0 and count as dead.
+  static __device__ __forceinline__ void request(Fetched& f, const AttnArgs& p, const int32_t* table, int64_t len, int64_t pos,
+                                                 int head, int lane) {
+    const int g = lane >> 4, c = lane & 15;
+    const int page_size = 1 << p.page_shift;
+    int64_t rows[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t first = pos + 16 * t;
+      int64_t page = first < len ? table[first >> p.page_shift] : 0;
+      f.valid[t] = first >= len ? 0 : (len - first < 16 ? (int) (len - first) : 16);
+      if (page < 0 || page >= p.n_pages) {
+        if (lane == 0) report(p.err, MI_IDERR_RANGE);
+        page = 0;
+        f.valid[t] = 0;
+      }
+      rows[t] = (((page * p.H + head) * 2) << p.page_shift) + (first & (page_size - 1));
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const char* kb = p.kv + rows[t] * (D * E);
@@ -403,13 +420,13 @@ struct Wave {
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const char* vb = p.kv + (rows[t] + page) * (D * E);
+      const char* vb = p.kv + (rows[t] + page_size) * (D * E);  // V lies page_size rows behind K
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int h = 0; h < VH; ++h)
           fetch<VB>(f.v[t][r][h], vb + (4 * g + r) * (D * E) + h * (VB * 16) + c * VB);
-      if (DT == MI_DT_E4M3) f.ev[t] = *reinterpret_cast<const unsigned int*>(p.exps + rows[t] + page + 4 * g);
+      if (DT == MI_DT_E4M3) f.ev[t] = *reinterpret_cast<const unsigned int*>(p.exps + rows[t] + page_size + 4 * g);
     }
   }
 
@@ -422,78 +439,107 @@ struct Wave {
     return __builtin_bit_cast(bf8v, w);
   }
 
-  // scores, softmax step and weighted sum of one chunk; valid[t]: live positions of tile t (16: all)
-  __device__ __forceinline__ void step(Fetched& f, const AttnArgs& p, const int (&valid)[2], int g, int c) {
-    f4v s[2];
+  // scores, softmax step and weighted sum of one chunk
+  __device__ __forceinline__ void step(Fetched& f, const AttnArgs& p, int lane) {
+    const int g = lane >> 4;
+    f4v s[RT][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      f4v acc = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < RT; ++i) s[i][t] = f4v{0.f, 0.f, 0.f, 0.f};
       if constexpr (F32) {
 #pragma unroll
         for (int k = 0; k < KL; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.k[t][k][i]), qv[k][i], acc, 0, 0, 0);
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+              s[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.k[t][k][e]), qv[i][k][e], s[i][t], 0, 0, 0);
       } else if constexpr (DT == MI_DT_BF16) {
 #pragma unroll
         for (int k = 0; k < KL; ++k) {
           const uint4 w = make_uint4(f.k[t][k][0], f.k[t][k][1], f.k[t][k][2], f.k[t][k][3]);
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, w), qf[k], acc, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+            s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, w), qf[i][k], s[i][t], 0, 0, 0);
         }
       } else {
 #pragma unroll
         for (int k = 0; k < KL; ++k)
 #pragma unroll
-          for (int u = 0; u < KB / 8; ++u)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(f.k[t][k][2 * u], f.k[t][k][2 * u + 1]),
-                                                          qf[k * (KB / 8) + u], acc, 0, 0, 0);
+          for (int u = 0; u < KB / 8; ++u) {
+            const bf8v w = widen(f.k[t][k][2 * u], f.k[t][k][2 * u + 1]);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+              s[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, qf[i][k * (KB / 8) + u], s[i][t], 0, 0, 0);
+          }
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = acc[r] * p.scale;
-        if (DT == MI_DT_E4M3) x *= pow2_bits((f.ek[t] >> (8 * r)) & 255u);
-        s[t][r] = x;
+        const float e = DT == MI_DT_E4M3 ? pow2_bits((f.ek[t] >> (8 * r)) & 255u) : 1.f;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          s[i][t][r] *= p.scale;
+          if (DT == MI_DT_E4M3) s[i][t][r] *= e;
+        }
       }
     }
-    if (valid[0] < 16 || valid[1] < 16) {  // the same in every lane: what lies behind the history is never used
+    if (f.valid[0] < 16 || f.valid[1] < 16) {  // the same in every lane: what lies behind the history is never used
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (4 * g + r >= valid[t]) {
-            s[t][r] = -INFINITY;
+          if (4 * g + r >= f.valid[t]) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) s[i][t][r] = -INFINITY;
 #pragma unroll
             for (int h = 0; h < VH; ++h)
 #pragma unroll
-              for (int i = 0; i < (VB < 4 ? 1 : VB / 4); ++i) f.v[t][r][h][i] = 0;
+              for (int e = 0; e < (VB < 4 ? 1 : VB / 4); ++e) f.v[t][r][h][e] = 0;
+            if (DT == MI_DT_E4M3) f.ev[t] &= ~(255u << (8 * r));  // a dead position's exponent is anything
           }
     }
-    float top = m;
+    float w[RT][8];
+    bf8v pf[RT];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int i = 0; i < RT; ++i) {
+      float top = m[i];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][r]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float base = top == -INFINITY ? 0.f : top;  // a row with no finite score yet: all weights are 0
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
-    m = top;
-    l *= alpha;
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int h = 0; h < VH; ++h)
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][t][r]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float base = top == -INFINITY ? 0.f : top;  // a row with no finite score yet: all weights are 0
+      const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
+      m[i] = top;
+      l[i] *= alpha;
 #pragma unroll
-      for (int j = 0; j < VE; ++j) o[h][j] *= alpha;
-    float w[8];
+      for (int h = 0; h < VH; ++h)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+        for (int j = 0; j < VE; ++j) o[i][h][j] *= alpha;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x = __builtin_amdgcn_exp2f(s[t][r] - base);
-        // 8- and 16-bit caches: the weights enter the product as bf16 (off by half a step, 2^-8 of the weight at most, as the output's own
-        // rounding is), and the sum they are divided by is that of the rounded weights
-        w[4 * t + r] = F32 ? x : (float) (__bf16) x;
-        l += w[4 * t + r];
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = __builtin_amdgcn_exp2f(s[i][t][r] - base);
+          // 8- and 16-bit caches: the weights enter the product as bf16 (off by half a step, 2^-8 of the weight at
+          // most, as the output's own rounding is), and the sum they are divided by is that of the rounded weights
+          w[i][4 * t + r] = F32 ? x : (float) (__bf16) x;
+          l[i] += w[i][4 * t + r];
+        }
+      if (!F32) {
+        if (DT == MI_DT_E4M3) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[i][4 * t + r] *= pow2_bits((f.ev[t] >> (8 * r)) & 255u);
+        }
+        const uint4 pw = make_uint4(pack_bf16(w[i][0], w[i][1]), pack_bf16(w[i][2], w[i][3]), pack_bf16(w[i][4], w[i][5]),
+                                    pack_bf16(w[i][6], w[i][7]));
+        pf[i] = __builtin_bit_cast(bf8v, pw);
       }
+    }
     if constexpr (F32) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -503,68 +549,53 @@ struct Wave {
           for (int h = 0; h < VH; ++h)
 #pragma unroll
             for (int j = 0; j < VE; ++j)
-              o[h][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[t][r][h][j]), w[4 * t + r], o[h][j], 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < RT; ++i)
+                o[i][h][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[t][r][h][j]), w[i][4 * t + r],
+                                                                  o[i][h][j], 0, 0, 0);
     } else {
-      if (DT == MI_DT_E4M3) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int h = 0; h < VH; ++h)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float e = pow2_bits((f.ev[t] >> (8 * r)) & 255u);
-            w[4 * t + r] *= 4 * g + r < valid[t] ? e : 0.f;  // a dead position's exponent is anything
-          }
-      }
-      uint4 pw;
-      pw.x = pack_bf16(w[0], w[1]);
-      pw.y = pack_bf16(w[2], w[3]);
-      pw.z = pack_bf16(w[4], w[5]);
-      pw.w = pack_bf16(w[6], w[7]);
-      const bf8v pf = __builtin_bit_cast(bf8v, pw);
+        for (int j = 0; j < VE; j += 2) {
+          uint4 a, b;  // channels j and j + 1 of the lane's eight positions
+          unsigned int* pa = &a.x;
+          unsigned int* pb = &b.x;
 #pragma unroll
-      for (int h = 0; h < VH; ++h) {
-        if constexpr (DT == MI_DT_BF16) {
-#pragma unroll
-          for (int j = 0; j < VE; j += 2) {
-            uint4 a, b;  // channels j and j + 1 of the lane's eight positions
-            unsigned int* pa = &a.x;
-            unsigned int* pb = &b.x;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (DT == MI_DT_BF16) {
               const unsigned int x = f.v[k >> 1][2 * (k & 1)][h][j / 2], y = f.v[k >> 1][2 * (k & 1) + 1][h][j / 2];
               pa[k] = __builtin_amdgcn_perm(y, x, 0x05040100u);
               pb[k] = __builtin_amdgcn_perm(y, x, 0x07060302u);
-            }
-            o[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), pf, o[h][j], 0, 0, 0);
-            o[h][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, b), pf, o[h][j + 1], 0, 0, 0);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < VE; j += 2) {
-            uint4 a, b;
-            unsigned int* pa = &a.x;
-            unsigned int* pb = &b.x;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            } else {
               const unsigned int x = f.v[k >> 1][2 * (k & 1)][h][j / 4], y = f.v[k >> 1][2 * (k & 1) + 1][h][j / 4];
               // bytes: channel j of both positions, then channel j + 1 of both
               const unsigned int z = __builtin_amdgcn_perm(y, x, (j & 2) ? 0x07030602u : 0x05010400u);
               pa[k] = __builtin_bit_cast(unsigned int, (bf2v) __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(z, 1.0f, false));
               pb[k] = __builtin_bit_cast(unsigned int, (bf2v) __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(z, 1.0f, true));
             }
-            o[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), pf, o[h][j], 0, 0, 0);
-            o[h][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, b), pf, o[h][j + 1], 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            o[i][h][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), pf[i], o[i][h][j], 0, 0, 0);
+            o[i][h][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, b), pf[i], o[i][h][j + 1], 0, 0, 0);
           }
         }
-      }
+    }
+  }
+
+  // row sums over the four g (every lane of a row ends with the same l)
+  __device__ __forceinline__ void close() {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      l[i] += __shfl_xor(l[i], 16, 64);
+      l[i] += __shfl_xor(l[i], 32, 64);
     }
   }
 
   // lane (g, c) holds channels h * (D / VH) + (4 g + r) * VE + j of query row c: contiguous in (r, j)
-  __device__ __forceinline__ void store(char* out_row, bool live, int g) {
-    float sum = l + __shfl_xor(l, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
-    if (!live) return;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  __device__ __forceinline__ void store(int t, char* out_row, int g) {
+    const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
 #pragma unroll
     for (int h = 0; h < VH; ++h) {
       char* dst = out_row + (h * (D / VH) + 4 * g * VE) * QE;
@@ -572,7 +603,7 @@ struct Wave {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) x[r * VE + j] = o[h][j][r] * inv;
+        for (int j = 0; j < VE; ++j) x[r * VE + j] = o[t][h][j][r] * inv;
       if constexpr (F32) {
 #pragma unroll
         for (int i = 0; i < 4 * VE; i += 4)
@@ -585,64 +616,321 @@ struct Wave {
       }
     }
   }
+
+  // unnormalised, in f32, for the joining launch: [D] sums, then m and l
+  __device__ __forceinline__ void store_part(int t, float* part_row, int g) {
+#pragma unroll
+    for (int h = 0; h < VH; ++h) {
+      float* dst = part_row + h * (D / VH) + 4 * g * VE;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VE; j += 2)
+          *reinterpret_cast<float2*>(dst + r * VE + j) = make_float2(o[t][h][j][r], o[t][h][j + 1][r]);
+    }
+    if (g == 0) *reinterpret_cast<float2*>(part_row + D) = make_float2(m[t], l[t]);
+  }
 };
 
-// One wave per (sequence, cache head, tile of 16 query rows).
-template <int DT, int D>
-__global__ __launch_bounds__(256) void hist_attn_kernel(AttnArgs p) {
-  typedef Wave<DT, D> W;
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-  const int64_t seg = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t pair = seg / p.n_rt;
-  const int rt = (int) (seg - pair * p.n_rt);
-  const int64_t b = pair / p.H;
-  const int head = (int) (pair - b * p.H);
-  if (b >= p.n_seqs) return;
+// The two halves of a pair of states, lane by lane the same rows and channels.
+struct Fold {
+  float a, b, m;
+};
+__device__ __forceinline__ Fold fold_of(float m1, float m2) {
+  const float top = fmaxf(m1, m2), base = top == -INFINITY ? 0.f : top;
+  return Fold{__builtin_amdgcn_exp2f(m1 - base), __builtin_amdgcn_exp2f(m2 - base), top};
+}
+
+// query row r of a cache head: token r / G, head r % G of the group
+template <int QE>
+__device__ __forceinline__ const char* q_row_of(const AttnArgs& p, int64_t b, int head, int row, bool live) {
+  const int tok = live ? row / p.G : 0, qh = head * p.G + (live ? row % p.G : 0);
+  return p.q + (b * p.q_seq + tok * p.q_tok + qh * p.q_head) * QE;
+}
+template <int QE>
+__device__ __forceinline__ char* out_row_of(const AttnArgs& p, int64_t b, int head, int row) {
+  return p.out + (b * p.o_seq + (row / p.G) * p.o_tok + (head * p.G + row % p.G) * p.o_head) * QE;
+}
+
+__device__ __forceinline__ int64_t clamped_length(const AttnArgs& p, int64_t b, bool say) {
   const int64_t room = (int64_t) p.width << p.page_shift;
-  int64_t len = p.lengths[b];
-  if (len > room) {
-    if (lane == 0) report(p.err, MI_IDERR_RANGE);
-    len = room;
-  }
+  const int64_t len = p.lengths[b];
+  if (len > room && say) report(p.err, MI_IDERR_RANGE);
+  return len > room ? room : (len < 0 ? 0 : len);
+}
+
+// Short histories: one wave per (sequence, cache head, tile of 16 query rows).
+template <int DT, int D>
+__global__ __launch_bounds__(256) void hist_attn_short_kernel(AttnArgs p) {
+  typedef Wave<DT, D, 1> W;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const unsigned int seg = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned int pair = seg / (unsigned int) p.n_rt;
+  const int rt = (int) (seg - pair * p.n_rt);
+  const int64_t b = pair / (unsigned int) p.H;
+  const int head = (int) (pair - (unsigned int) b * p.H);
+  if (b >= p.n_seqs) return;
+  const int64_t len = clamped_length(p, b, lane == 0);
   const int row = rt * 16 + c;
   const bool live = row < p.rows;
-  const int tok = live ? row / p.G : 0, qh = head * p.G + (live ? row % p.G : 0);
   W w;
-  w.init(p.q + (b * p.q_seq + tok * p.q_tok + qh * p.q_head) * W::QE, live, g);
+  w.init(0, q_row_of<W::QE>(p, b, head, row, live), live, g);
   const int32_t* table = p.table + b * p.ld_table;
   for (int64_t pos = 0; pos < len; pos += W::CHUNK) {
-    int64_t rows[2];
-    int valid[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int64_t first = pos + 16 * t;
-      int64_t page = first < len ? table[first >> p.page_shift] : 0;
-      valid[t] = first >= len ? 0 : (len - first < 16 ? (int) (len - first) : 16);
-      if (page < 0 || page >= p.n_pages) {
-        if (lane == 0) report(p.err, MI_IDERR_RANGE);
-        page = 0;
-        valid[t] = 0;
-      }
-      rows[t] = (((page * p.H + head) * 2) << p.page_shift) + (first & ((1 << p.page_shift) - 1));
-    }
     typename W::Fetched f;
-    w.request(f, p, rows, g, c);
-    w.step(f, p, valid, g, c);
+    W::request(f, p, table, len, pos, head, lane);
+    w.step(f, p, lane);
   }
-  w.store(p.out + (b * p.o_seq + tok * p.o_tok + qh * p.o_head) * W::QE, live, g);
+  w.close();
+  if (live) w.store(0, out_row_of<W::QE>(p, b, head, row), g);
+}
+
+// Long histories: the call's work is cut into equal runs of units, a unit being UNIT positions of one (sequence, cache
+// head, group of query rows), sequences slowest; a workgroup walks its run.  A run that begins or ends inside a
+// (sequence, head, group) leaves an unnormalised part, which the joining launch adds up.  The cut goes by the lengths
+// alone, so histories of any mix keep every workgroup equally busy, and the parts are always joined in the same order.
+constexpr int UNIT = 128;
+
+struct SplitArgs {
+  int NR;            // row tiles side by side in a workgroup: 1, 2 or 4 waves; the other waves share the positions
+  int NG;            // groups of NR * 16 * RT query rows
+  int min_run;       // units a workgroup takes at least
+  float* parts;      // [workgroups][2][NR * 16 * RT][D + 4]
+  int4* meta;        // [workgroups] {sequence (-1: nothing to join), head * NG + group, last workgroup, 0}
+};
+
+__device__ __forceinline__ unsigned int units_of(int64_t len) {
+  return len <= UNIT ? 1u : (unsigned int) ((len + UNIT - 1) / UNIT);
+}
+
+template <int DT, int D, int RT>
+__global__ __launch_bounds__(256) void hist_attn_split_kernel(AttnArgs p, SplitArgs a) {
+  typedef Wave<DT, D, RT> W;
+  __shared__ f4v lo[2][RT * W::VH * W::VE][64];
+  __shared__ float2 lml[2][RT][64];
+  __shared__ unsigned int wave_sum[4];
+  __shared__ unsigned int found[2];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned int HG = (unsigned int) (p.H * a.NG), n_seqs = (unsigned int) p.n_seqs;
+
+  // units in front of each thread's slice of the sequences
+  const unsigned int per = (n_seqs + 255) / 256;
+  const unsigned int s0 = threadIdx.x * per, s1 = s0 + per < n_seqs ? s0 + per : n_seqs;
+  unsigned int mine = 0;
+  for (unsigned int b = s0; b < s1; ++b) mine += units_of(clamped_length(p, b, blockIdx.x == 0));
+  unsigned int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned int up = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 63) wave_sum[wave] = incl;
+  __syncthreads();
+  unsigned int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < wave) before += wave_sum[i];
+    all += wave_sum[i];
+  }
+  before += incl - mine;
+  const unsigned int total = all * HG;  // < 2^31, checked on the host
+  unsigned int run = (total + gridDim.x - 1) / gridDim.x;
+  if (run < (unsigned int) a.min_run) run = (unsigned int) a.min_run;
+  const unsigned int x0 = blockIdx.x * run, x1 = x0 + run < total ? x0 + run : total;
+  if (x0 < total && before * HG <= x0 && x0 < (before + mine) * HG) {
+    unsigned int b = s0;
+    for (;; ++b) {
+      const unsigned int u = units_of(clamped_length(p, b, false));
+      if (x0 < (before + u) * HG) break;
+      before += u;
+    }
+    found[0] = b;
+    found[1] = before * HG;
+  }
+  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  __syncthreads();
+  if (x0 >= total) return;
+
+  const int rt = wave % a.NR, ci = wave / a.NR, CI = 4 / a.NR;
+  const int group_rows = a.NR * 16 * RT;
+  const int part_ld = D + 4;
+  unsigned int b = __builtin_amdgcn_readfirstlane(found[0]);
+  unsigned int start = __builtin_amdgcn_readfirstlane(found[1]);
+  unsigned int x = x0;
+  while (x < x1) {
+    const int64_t len = clamped_length(p, b, false);
+    const unsigned int u = units_of(len);
+    const unsigned int rem = x - start, pair = rem / u, ub = rem - pair * u;
+    const int head = (int) (pair / (unsigned int) a.NG), grp = (int) (pair - (unsigned int) head * a.NG);
+    const unsigned int ue = ub + (x1 - x) < u ? ub + (x1 - x) : u;
+    const int row0 = (grp * a.NR + rt) * 16 * RT;
+    W w;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = row0 + t * 16 + c;
+      w.init(t, q_row_of<W::QE>(p, b, head, row, row < p.rows), row < p.rows, g);
+    }
+    const int32_t* table = p.table + (int64_t) b * p.ld_table;
+    const int64_t end = (int64_t) ue * UNIT < len ? (int64_t) ue * UNIT : len;
+    if (row0 < p.rows) {
+      for (int64_t pos = (int64_t) ub * UNIT + ci * W::CHUNK; pos < end; pos += CI * W::CHUNK) {
+        typename W::Fetched f;
+        W::request(f, p, table, len, pos, head, lane);
+        w.step(f, p, lane);
+      }
+    }
+    w.close();
+    // the waves that shared the positions of a row tile: halves fold together, lane by lane
+    for (int half = CI >> 1; half > 0; half >>= 1) {
+      const int slot = (ci - half) * a.NR + rt;  // < 2: half * NR <= 2
+      if (ci >= half && ci < 2 * half) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          lml[slot][t][lane] = make_float2(w.m[t], w.l[t]);
+#pragma unroll
+          for (int i = 0; i < W::VH * W::VE; ++i) lo[slot][t * W::VH * W::VE + i][lane] = w.o[t][i / W::VE][i % W::VE];
+        }
+      }
+      __syncthreads();
+      if (ci < half) {
+        const int from = ci * a.NR + rt;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const float2 ml = lml[from][t][lane];
+          const Fold k = fold_of(w.m[t], ml.x);
+          w.m[t] = k.m;
+          w.l[t] = w.l[t] * k.a + ml.y * k.b;
+#pragma unroll
+          for (int i = 0; i < W::VH * W::VE; ++i)
+            w.o[t][i / W::VE][i % W::VE] = w.o[t][i / W::VE][i % W::VE] * k.a + lo[from][t * W::VH * W::VE + i][lane] * k.b;
+        }
+      }
+      __syncthreads();
+    }
+    if (ci == 0) {
+      const bool whole = ub == 0 && ue == u;
+      float* part = a.parts + ((int64_t) blockIdx.x * 2 + (ub == 0 ? 1 : 0)) * group_rows * part_ld;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int row = row0 + t * 16 + c;
+        if (row < p.rows) {
+          if (whole) w.store(t, out_row_of<W::QE>(p, b, head, row), g);
+          else w.store_part(t, part + (int64_t) (row - grp * group_rows) * part_ld, g);
+        }
+      }
+      if (threadIdx.x == 0 && ub == 0 && ue < u)
+        a.meta[blockIdx.x] = make_int4((int) b, (int) pair, (int) ((x + u - 1) / run), 0);
+    }
+    x += ue - ub;
+    if (ue == u && pair + 1 == HG) {
+      start += u * HG;
+      ++b;
+    }
+  }
+}
+
+// Joins the parts of the (sequence, head, group) that workgroup blockIdx.x began and did not finish: its own second
+// part, then the first parts of the workgroups behind it, in order.  A wave per query row.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void hist_attn_join_kernel(AttnArgs p, SplitArgs a, int group_rows) {
+  constexpr int QE = DT == MI_DT_F32 ? 4 : 2;
+  const int4 meta = a.meta[blockIdx.x];
+  if (meta.x < 0) return;
+  const int lane = threadIdx.x & 63;
+  const int head = meta.y / a.NG, grp = meta.y % a.NG;
+  const int n = meta.z - (int) blockIdx.x + 1;
+  const int part_ld = D + 4;
+  const int64_t slot = (int64_t) group_rows * part_ld;
+  for (int r = threadIdx.x >> 6; r < group_rows && grp * group_rows + r < p.rows; r += 4) {
+    const float* first = a.parts + ((int64_t) blockIdx.x * 2 + 1) * slot + (int64_t) r * part_ld;
+    const float* rest = a.parts + (int64_t) blockIdx.x * 2 * slot + (int64_t) r * part_ld;  // + 2 * slot * i
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, (i ? rest + 2 * slot * i : first)[D]);
+    top = mi_wave_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    constexpr int CPL = D >= 64 ? D / 64 : 1;
+    float acc[CPL], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) acc[j] = 0.f;
+    const int d = (lane * CPL) & (D - 1);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float* part = i ? rest + 2 * slot * i : first;
+      const float2 ml = *reinterpret_cast<const float2*>(part + D);
+      const float k = __builtin_amdgcn_exp2f(ml.x - base);
+      sum += ml.y * k;
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) acc[j] += part[d + j] * k;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    char* out = out_row_of<QE>(p, meta.x, head, grp * group_rows + r) + d * QE;
+    if (lane * CPL < D) {
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) {
+        if (DT == MI_DT_F32) reinterpret_cast<float*>(out)[j] = acc[j] * inv;
+        else reinterpret_cast<unsigned short*>(out)[j] = mi_f2bf(acc[j] * inv);
+      }
+    }
+  }
+}
+
+// How a call is run; the same on every call of the same sizes.
+struct AttnPlan {
+  bool short_rows;
+  int RT, NR, NG, blocks, min_run;
+  size_t parts_bytes, bytes;
+};
+
+AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int64_t rows, int width) {
+  AttnPlan q = {};
+  const int64_t room = (int64_t) width * page_size;
+  q.RT = rows > 16 && dim <= 128 ? 2 : 1;  // two tiles of 256 channels do not fit the registers
+  const int64_t tiles = mi_cdiv(rows, 16 * q.RT);
+  q.NR = tiles >= 3 ? 4 : (int) tiles;
+  q.NG = (int) mi_cdiv(tiles, q.NR);
+  q.short_rows = room <= 256;
+  q.min_run = 1;
+  const int64_t most = n_seqs * H * q.NG * mi_cdiv(room, UNIT);
+  const int64_t resident = 1024;
+  q.blocks = (int) (most < resident ? most : resident);
+  if (!q.short_rows) {
+    q.parts_bytes = (size_t) q.blocks * 2 * q.NR * 16 * q.RT * (dim + 4) * sizeof(float);
+    q.bytes = q.parts_bytes + (size_t) q.blocks * sizeof(int4);
+  }
+  (void) dtype;
+  return q;
+}
+
+template <int DT, int D>
+int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) {
+  if (q.short_rows) {
+    hist_attn_short_kernel<DT, D><<<dim3((unsigned int) mi_cdiv(p.n_seqs * p.H * p.n_rt, 4)), 256, 0, s>>>(p);
+    MI_LAUNCH_CHECK();
+    return MI_OK;
+  }
+  SplitArgs a = {};
+  a.NR = q.NR;
+  a.NG = q.NG;
+  a.min_run = q.min_run;
+  a.parts = (float*) ws;
+  a.meta = (int4*) ((char*) ws + q.parts_bytes);
+  if (q.RT == 2) hist_attn_split_kernel<DT, D, D <= 128 ? 2 : 1><<<q.blocks, 256, 0, s>>>(p, a);
+  else hist_attn_split_kernel<DT, D, 1><<<q.blocks, 256, 0, s>>>(p, a);
+  MI_LAUNCH_CHECK();
+  hist_attn_join_kernel<DT, D><<<q.blocks, 256, 0, s>>>(p, a, q.NR * 16 * q.RT);
+  MI_LAUNCH_CHECK();
+  return MI_OK;
 }
 
 template <int DT>
-int launch_attn(const AttnArgs& p, int dim, hipStream_t s) {
-  const dim3 grid((unsigned int) mi_cdiv(p.n_seqs * p.H * p.n_rt, 4));
+int launch_attn(const AttnArgs& p, const AttnPlan& q, int dim, void* ws, hipStream_t s) {
   switch (dim) {
-    case 32: hist_attn_kernel<DT, 32><<<grid, 256, 0, s>>>(p); break;
-    case 64: hist_attn_kernel<DT, 64><<<grid, 256, 0, s>>>(p); break;
-    case 128: hist_attn_kernel<DT, 128><<<grid, 256, 0, s>>>(p); break;
-    default: hist_attn_kernel<DT, 256><<<grid, 256, 0, s>>>(p); break;
+    case 32: return launch_attn_dim<DT, 32>(p, q, ws, s);
+    case 64: return launch_attn_dim<DT, 64>(p, q, ws, s);
+    case 128: return launch_attn_dim<DT, 128>(p, q, ws, s);
+    default: return launch_attn_dim<DT, 256>(p, q, ws, s);
   }
-  MI_LAUNCH_CHECK();
-  return MI_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ host checks
@@ -757,20 +1045,17 @@ extern "C" int mi_hist_read(const mi_hist_cache* cache, void* k, void* v, int dt
 
 extern "C" size_t mi_hist_attn_workspace_bytes(const mi_hist_cache* cache, int64_t n_seqs, int n_queries, int q_heads,
                                                int table_width) {
-  (void) cache;
-  (void) n_seqs;
-  (void) n_queries;
-  (void) q_heads;
-  (void) table_width;
-  return 0;
+  if (check_cache(cache, "mi_hist_attn_workspace_bytes") || n_seqs < 1 || n_queries < 1 || q_heads < 1 || table_width < 1 ||
+      q_heads % cache->n_heads)
+    return 0;
+  return plan_attn(cache->dtype, cache->dim, cache->n_heads, cache->page_size, n_seqs,
+                   (int64_t) n_queries * (q_heads / cache->n_heads), table_width).bytes;
 }
 
 extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q_seq, int64_t q_tok, int64_t q_head, int q_heads,
                             int n_queries, int64_t n_seqs, const int32_t* page_table, int64_t ld_table, int table_width,
                             const int32_t* lengths, float scale, void* out, int64_t out_seq, int64_t out_tok, int64_t out_head,
                             void* workspace, size_t workspace_bytes, int32_t* err, void* stream) {
-  (void) workspace;
-  (void) workspace_bytes;
   if (int rc = check_cache(cache, "mi_hist_attn")) return rc;
   MI_REQUIRE(n_queries >= 0 && q_heads >= 1 && q_heads % cache->n_heads == 0,
              "mi_hist_attn: %d queries of %d heads over a cache of %d heads", n_queries, q_heads, cache->n_heads);
@@ -806,14 +1091,24 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
   p.n_seqs = n_seqs;
   p.scale = scale * 1.44269504088896340736f;
   p.err = err;
-  if (n_seqs * p.H * p.n_rt > (int64_t) INT32_MAX) {
-    mi_set_error("mi_hist_attn: %lld sequences x %d heads x %d row tiles in one call", (long long) n_seqs, p.H, p.n_rt);
+  const AttnPlan plan = plan_attn(cache->dtype, cache->dim, p.H, cache->page_size, n_seqs, rows, table_width);
+  // unit and segment numbers are 32-bit in the kernels
+  if (mi_cdiv((int64_t) table_width * cache->page_size, UNIT) > INT32_MAX / (n_seqs * p.H) / p.n_rt) {
+    mi_set_error("mi_hist_attn: %lld sequences x %d heads x %d row tiles over %d pages in one call", (long long) n_seqs, p.H,
+                 p.n_rt, table_width);
     return MI_ERR_UNSUPPORTED;
+  }
+  if (plan.bytes) {
+    MI_REQUIRE(((uintptr_t) workspace & 15) == 0, "mi_hist_attn: the workspace must be 16-byte aligned");
+    if (!workspace || workspace_bytes < plan.bytes) {
+      mi_set_error("mi_hist_attn: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t) 0, plan.bytes);
+      return MI_ERR_WORKSPACE;
+    }
   }
   hipStream_t s = (hipStream_t) stream;
   switch (cache->dtype) {
-    case MI_DT_F32: return launch_attn<MI_DT_F32>(p, cache->dim, s);
-    case MI_DT_BF16: return launch_attn<MI_DT_BF16>(p, cache->dim, s);
-    default: return launch_attn<MI_DT_E4M3>(p, cache->dim, s);
+    case MI_DT_F32: return launch_attn<MI_DT_F32>(p, plan, cache->dim, workspace, s);
+    case MI_DT_BF16: return launch_attn<MI_DT_BF16>(p, plan, cache->dim, workspace, s);
+    default: return launch_attn<MI_DT_E4M3>(p, plan, cache->dim, workspace, s);
   }
 }

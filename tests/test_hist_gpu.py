@@ -315,7 +315,9 @@ def test_bad_pages_are_absent_and_reported(dev, cache):
     err = ops.new_error_word(dev)
     got2 = ops.hist_attn(c, q[2:3], table[2:3, :4], torch.tensor([70], dtype=torch.int32, device=dev), err=err)
     assert err.item() == 1
-    np.testing.assert_array_equal(got2.double().cpu().numpy()[0], got[2])
+    # (a narrower table may be summed in another order: held to the definition, not to the call above)
+    held("hist_attn %s beyond the table" % cache,
+         (np.abs(got2.double().cpu().numpy() - want[2:3]) / bound(cache, 64, 64, want, absv, size)[2:3]).max(), 1.0)
     ops.hist_attn(c, q[2:3], table[2:3, :4], torch.tensor([64], dtype=torch.int32, device=dev), err=ops.new_error_word(dev))
 
 
