@@ -831,41 +831,92 @@ __global__ __launch_bounds__(256) void hist_attn_split_kernel(AttnArgs p, SplitA
 }
 
 // Joins the parts of the (sequence, head, group) that workgroup blockIdx.x began and did not finish: its own second
-// part, then the first parts of the workgroups behind it, in order.  A wave per query row.
+// part, then the first parts of the workgroups behind it, in order.  JOIN_WAVES query rows per workgroup, a wave each;
+// of fewer rows several waves take a run of the parts each.
+constexpr int JOIN_WAVES = 4;
+
 template <int DT, int D>
-__global__ __launch_bounds__(256) void hist_attn_join_kernel(AttnArgs p, SplitArgs a, int group_rows) {
+__global__ __launch_bounds__(JOIN_WAVES * 64) void hist_attn_join_kernel(AttnArgs p, SplitArgs a, int group_rows) {
   constexpr int QE = DT == MI_DT_F32 ? 4 : 2;
+  constexpr int CPL = D >= 64 ? D / 64 : 1;  // channels per lane
+  __shared__ float lacc[JOIN_WAVES][D];
+  __shared__ float2 lml[JOIN_WAVES];
   const int4 meta = a.meta[blockIdx.x];
   if (meta.x < 0) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = meta.y / a.NG, grp = meta.y % a.NG;
   const int n = meta.z - (int) blockIdx.x + 1;
   const int part_ld = D + 4;
   const int64_t slot = (int64_t) group_rows * part_ld;
-  for (int r = threadIdx.x >> 6; r < group_rows && grp * group_rows + r < p.rows; r += 4) {
-    const float* first = a.parts + ((int64_t) blockIdx.x * 2 + 1) * slot + (int64_t) r * part_ld;
-    const float* rest = a.parts + (int64_t) blockIdx.x * 2 * slot + (int64_t) r * part_ld;  // + 2 * slot * i
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, (i ? rest + 2 * slot * i : first)[D]);
-    top = mi_wave_max(top);
-    const float base = top == -INFINITY ? 0.f : top;
-    constexpr int CPL = D >= 64 ? D / 64 : 1;
-    float acc[CPL], sum = 0.f;
+  const int n_rows = p.rows - grp * group_rows < group_rows ? p.rows - grp * group_rows : group_rows;
+  const int r0 = (int) blockIdx.y * JOIN_WAVES;
+  if (r0 >= n_rows) return;
+  int side = 1;  // rows side by side, a power of two
+  while (side < n_rows - r0 && side < JOIN_WAVES) side <<= 1;
+  const int runs = JOIN_WAVES / side, mine = wave / side;
+  const int per = (n + runs - 1) / runs;
+  const int i0 = mine * per, i1 = i0 + per < n ? i0 + per : n;
+  const int d = (lane * CPL) & (D - 1);
+  {
+    const int r = r0 + wave % side;
+    const bool live = r < n_rows;
+    float top = -INFINITY, sum = 0.f, acc[CPL];
 #pragma unroll
     for (int j = 0; j < CPL; ++j) acc[j] = 0.f;
-    const int d = (lane * CPL) & (D - 1);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float* part = i ? rest + 2 * slot * i : first;
-      const float2 ml = *reinterpret_cast<const float2*>(part + D);
-      const float k = __builtin_amdgcn_exp2f(ml.x - base);
-      sum += ml.y * k;
+    if (live) {
+      const float* first = a.parts + ((int64_t) blockIdx.x * 2 + 1) * slot + (int64_t) r * part_ld;
+      const float* rest = a.parts + (int64_t) blockIdx.x * 2 * slot + (int64_t) r * part_ld;  // part i > 0: + 2 slot i
+      for (int i = i0 + lane; i < i1; i += 64) top = fmaxf(top, (i ? rest + 2 * slot * i : first)[D]);
+      top = mi_wave_max(top);
+      const float base = top == -INFINITY ? 0.f : top;
+      for (int ib = i0; ib < i1; ib += 64) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (ib + lane < i1) ml = *reinterpret_cast<const float2*>((ib + lane ? rest + 2 * slot * (ib + lane) : first) + D);
+        const float k = __builtin_amdgcn_exp2f(ml.x - base);
+        sum += ml.y * k;
+        const int m = i1 - ib < 64 ? i1 - ib : 64;
+        // eight parts requested together; behind the last one the last again, unused
+        for (int i = 0; i < m; i += 8) {
+          float x[8][CPL];
 #pragma unroll
-      for (int j = 0; j < CPL; ++j) acc[j] += part[d + j] * k;
+          for (int e = 0; e < 8; ++e) {
+            const int at = ib + (i + e < m ? i + e : m - 1);
+            const float* part = at ? rest + 2 * slot * at : first;
+#pragma unroll
+            for (int j = 0; j < CPL; ++j) x[e][j] = part[d + j];
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float ke = i + e < m ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k), (i + e) & 63)) : 0.f;
+#pragma unroll
+            for (int j = 0; j < CPL; ++j) acc[j] = i + e < m ? acc[j] + x[e][j] * ke : acc[j];
+          }
+        }
+      }
+      sum = mi_wave_sum(sum);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    char* out = out_row_of<QE>(p, meta.x, head, grp * group_rows + r) + d * QE;
-    if (lane * CPL < D) {
+    if (runs > 1) {
+      if (lane * CPL < D) {
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) lacc[wave][d + j] = acc[j];
+      }
+      if (lane == 0) lml[wave] = make_float2(top, sum);
+      __syncthreads();
+      if (mine == 0) {
+        for (int k = 1; k < runs; ++k) {
+          const int from = wave + k * side;
+          const float m1 = top, m2 = lml[from].x, m = fmaxf(m1, m2), base = m == -INFINITY ? 0.f : m;
+          const float f1 = __builtin_amdgcn_exp2f(m1 - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+          top = m;
+          sum = sum * f1 + lml[from].y * f2;
+#pragma unroll
+          for (int j = 0; j < CPL; ++j) acc[j] = acc[j] * f1 + lacc[from][d + j] * f2;
+        }
+      }
+    }
+    if (live && mine == 0 && lane * CPL < D) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      char* out = out_row_of<QE>(p, meta.x, head, grp * group_rows + r) + d * QE;
 #pragma unroll
       for (int j = 0; j < CPL; ++j) {
         if (DT == MI_DT_F32) reinterpret_cast<float*>(out)[j] = acc[j] * inv;
@@ -874,6 +925,9 @@ __global__ __launch_bounds__(256) void hist_attn_join_kernel(AttnArgs p, SplitAr
     }
   }
 }
+
+// Workgroups of the split kernel on one CU (a wave on each SIMD): what its registers allow, asked of the compiler.
+constexpr int split_waves(int dim, int RT) { return dim <= 64 ? (RT == 1 ? 4 : 3) : dim == 128 ? 2 : 1; }
 
 // How a call is run; the same on every call of the same sizes.
 struct AttnPlan {
@@ -892,7 +946,7 @@ AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int
   q.short_rows = room <= 256;
   q.min_run = 1;
   const int64_t most = n_seqs * H * q.NG * mi_cdiv(room, UNIT);
-  const int64_t resident = 1024;
+  const int64_t resident = 256 * split_waves(dim, q.RT);
   q.blocks = (int) (most < resident ? most : resident);
   if (!q.short_rows) {
     q.parts_bytes = (size_t) q.blocks * 2 * q.NR * 16 * q.RT * (dim + 4) * sizeof(float);
@@ -918,7 +972,9 @@ int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t 
   if (q.RT == 2) hist_attn_split_kernel<DT, D, D <= 128 ? 2 : 1><<<q.blocks, 256, 0, s>>>(p, a);
   else hist_attn_split_kernel<DT, D, 1><<<q.blocks, 256, 0, s>>>(p, a);
   MI_LAUNCH_CHECK();
-  hist_attn_join_kernel<DT, D><<<q.blocks, 256, 0, s>>>(p, a, q.NR * 16 * q.RT);
+  const int group_rows = q.NR * 16 * q.RT;
+  const dim3 grid(q.blocks, (unsigned int) mi_cdiv(p.rows < group_rows ? p.rows : group_rows, JOIN_WAVES));
+  hist_attn_join_kernel<DT, D><<<grid, JOIN_WAVES * 64, 0, s>>>(p, a, group_rows);
   MI_LAUNCH_CHECK();
   return MI_OK;
 }
