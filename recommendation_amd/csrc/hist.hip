@@ -30,6 +30,21 @@ struct Elem<MI_DT_E4M3> {
   static constexpr int BYTES = 1;
 };
 
+// over the lanes l, l ^ 16, l ^ 32, l ^ 48: the swaps leave both halves of a pair in both results
+__device__ __forceinline__ float max_over_g(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Read-only memory at a wave-uniform address, through the scalar cache (the compiler cannot know that nothing in the
+// launch writes it, and a vector load in its place would have to wait for every load in flight).
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+  return *(const __attribute__((address_space(4))) T*) (p);
+}
+
 __device__ __forceinline__ float pow2_bits(unsigned int e) { return __uint_as_float(e << 23); }
 
 __device__ __forceinline__ void report(int32_t* err, int bit) {
@@ -321,6 +336,11 @@ struct AttnArgs {
 // its right operand if its reduction index is read as "positions 4g..4g+3 of tile 0, then of tile 1".  Its left
 // operand takes output channels j of 16 lanes' 16-byte pieces of a V row, whatever those channels are called.  So no
 // score, probability or value crosses lanes; only the row maximum and sum do (over the four g).
+// Waves on a SIMD, asked of the compiler (registers) and counted on when the work is cut.
+constexpr int split_waves(bool f32, int dim, int RT) {
+  return dim == 256 ? 1 : dim == 128 ? (f32 && RT == 2 ? 1 : 2) : dim == 64 ? (f32 ? 3 : 4) - (RT - 1) : 4 - (RT - 1);
+}
+
 template <int DT, int D, int RT>
 struct Wave {
   static constexpr bool F32 = DT == MI_DT_F32;
@@ -336,6 +356,7 @@ struct Wave {
   static constexpr int VH = D / 16 / VE;
   static constexpr int CHUNK = 32;                          // positions per step, two tiles
   static constexpr int NS = D / 32;                         // 32-channel steps of the score product (8 / 16 bit)
+  static constexpr float SLACK = 8.f;
 
   f4v o[RT][VH][VE];
   float m[RT], l[RT];
@@ -374,7 +395,6 @@ struct Wave {
     unsigned int k[2][KL][KB / 4];
     unsigned int v[2][4][VH][VB < 4 ? 1 : VB / 4];
     unsigned int ek[2], ev[2];
-    int valid[2];                                           // live positions of each tile, the same in every lane
   };
 
   template <int BYTES>
@@ -392,41 +412,82 @@ struct Wave {
     }
   }
 
-  // Requests the 32 positions from `pos` of a history of `len` (table: the sequence's pages).  Tiles behind the end,
-  // or on a bad page, read page 0 and count as dead.
-  static __device__ __forceinline__ void request(Fetched& f, const AttnArgs& p, const int32_t* table, int64_t len, int64_t pos,
-                                                 int head, int lane) {
-    const int g = lane >> 4, c = lane & 15;
-    const int page_size = 1 << p.page_shift;
+  // A chunk's two tiles: first K row of each in the cache, and how many positions are live (both wave-uniform).
+  struct Where {
     int64_t rows[2];
+    int valid[2];
+  };
+  // The 32 positions from `pos` of a history walked up to `len` (table: the sequence's pages).  Tiles behind, or on a bad
+  // page, count as dead and stand at page 0; a chunk that lies behind the end as a whole stands where `last` does.
+  static __device__ __forceinline__ Where locate(const AttnArgs& p, const int32_t* table, int64_t len, int64_t pos, int head,
+                                                 const Where& last, int lane) {
+    Where w = last;
+    w.valid[0] = w.valid[1] = 0;
+    if (pos < len) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int64_t first = pos + 16 * t;
-      int64_t page = first < len ? table[first >> p.page_shift] : 0;
-      f.valid[t] = first >= len ? 0 : (len - first < 16 ? (int) (len - first) : 16);
-      if (page < 0 || page >= p.n_pages) {
-        if (lane == 0) report(p.err, MI_IDERR_RANGE);
-        page = 0;
-        f.valid[t] = 0;
+      for (int t = 0; t < 2; ++t) {
+        const int64_t first = pos + 16 * t;
+        int64_t page = first < len ? scalar_load(table + (first >> p.page_shift)) : 0;
+        w.valid[t] = first >= len ? 0 : (len - first < 16 ? (int) (len - first) : 16);
+        if (page < 0 || page >= p.n_pages) {
+          if (lane == 0) report(p.err, MI_IDERR_RANGE);
+          page = 0;
+          w.valid[t] = 0;
+        }
+        w.rows[t] = (((page * p.H + head) * 2) << p.page_shift) + (first & ((1 << p.page_shift) - 1));
       }
-      rows[t] = (((page * p.H + head) * 2) << p.page_shift) + (first & (page_size - 1));
     }
+    return w;
+  }
+  static __device__ __forceinline__ void request_k(Fetched& f, const AttnArgs& p, const Where& w, int lane) {
+    const int g = lane >> 4, c = lane & 15;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const char* kb = p.kv + rows[t] * (D * E);
+      const char* kb = p.kv + w.rows[t] * (D * E);
 #pragma unroll
       for (int s = 0; s < KL; ++s) fetch<KB>(f.k[t][s], kb + c * (D * E) + s * (KB * 4) + g * KB);
-      if (DT == MI_DT_E4M3) f.ek[t] = *reinterpret_cast<const unsigned int*>(p.exps + rows[t] + 4 * g);
+      if (DT == MI_DT_E4M3) f.ek[t] = *reinterpret_cast<const unsigned int*>(p.exps + w.rows[t] + 4 * g);
     }
+    __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the work they are to overlap
+  }
+  static __device__ __forceinline__ void request_v(Fetched& f, const AttnArgs& p, const Where& w, int lane) {
+    const int g = lane >> 4, c = lane & 15;
+    const int page_size = 1 << p.page_shift;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const char* vb = p.kv + (rows[t] + page_size) * (D * E);  // V lies page_size rows behind K
+      const char* vb = p.kv + (w.rows[t] + page_size) * (D * E);  // V lies page_size rows behind K
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int h = 0; h < VH; ++h)
           fetch<VB>(f.v[t][r][h], vb + (4 * g + r) * (D * E) + h * (VB * 16) + c * VB);
-      if (DT == MI_DT_E4M3) f.ev[t] = *reinterpret_cast<const unsigned int*>(p.exps + rows[t] + page_size + 4 * g);
+      if (DT == MI_DT_E4M3) f.ev[t] = *reinterpret_cast<const unsigned int*>(p.exps + w.rows[t] + page_size + 4 * g);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // All chunks pos, pos + stride, ... < end.  A chunk's K is requested while the values of the one before are summed,
+  // its V while its own scores are formed: one set of registers, and loads in flight all the time.  Behind the end the
+  // last chunk is requested again (from the caches): a load that some steps skip would make every step wait for all.
+  __device__ __forceinline__ void walk(const AttnArgs& p, const int32_t* table, int64_t pos, int64_t end, int64_t stride,
+                                       int head, int lane) {
+    if (pos >= end) return;
+    Fetched f;
+    Where at, next;
+    at.rows[0] = at.rows[1] = 0;
+    at = locate(p, table, end, pos, head, at, lane);
+    request_k(f, p, at, lane);
+    request_v(f, p, at, lane);
+    for (;;) {
+      next = locate(p, table, end, pos + stride, head, at, lane);
+      f4v s[RT][2];
+      scores(s, f, p);
+      request_k(f, p, next, lane);
+      weigh(s, f, at, lane);
+      request_v(f, p, next, lane);
+      pos += stride;
+      if (pos >= end) break;
+      at = next;
     }
   }
 
@@ -439,10 +500,8 @@ struct Wave {
     return __builtin_bit_cast(bf8v, w);
   }
 
-  // scores, softmax step and weighted sum of one chunk
-  __device__ __forceinline__ void step(Fetched& f, const AttnArgs& p, int lane) {
-    const int g = lane >> 4;
-    f4v s[RT][2];
+  // scores of one chunk, times log2(e)
+  __device__ __forceinline__ void scores(f4v (&s)[RT][2], const Fetched& f, const AttnArgs& p) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -484,12 +543,17 @@ struct Wave {
         }
       }
     }
-    if (f.valid[0] < 16 || f.valid[1] < 16) {  // the same in every lane: what lies behind the history is never used
+  }
+
+  // softmax step and weighted sum of one chunk
+  __device__ __forceinline__ void weigh(f4v (&s)[RT][2], Fetched& f, const Where& at, int lane) {
+    const int g = lane >> 4;
+    if (at.valid[0] < 16 || at.valid[1] < 16) {  // the same in every lane: what lies behind the history is never used
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (4 * g + r >= f.valid[t]) {
+          if (4 * g + r >= at.valid[t]) {
 #pragma unroll
             for (int i = 0; i < RT; ++i) s[i][t][r] = -INFINITY;
 #pragma unroll
@@ -508,36 +572,42 @@ struct Wave {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][t][r]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float base = top == -INFINITY ? 0.f : top;  // a row with no finite score yet: all weights are 0
-      const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
-      m[i] = top;
-      l[i] *= alpha;
+      top = max_over_g(top);
+      // m is a score that the row's weights are taken against, at most SLACK below its maximum so far: most chunks
+      // then leave the sums as they are, at weights of up to 2^SLACK
+      if (__any(top > m[i] + SLACK)) {
+        const float up = top > m[i] + SLACK ? top : m[i];
+        const float alpha = up == m[i] ? 1.f : __builtin_amdgcn_exp2f(m[i] - up);
+        m[i] = up;
+        l[i] *= alpha;
 #pragma unroll
-      for (int h = 0; h < VH; ++h)
+        for (int h = 0; h < VH; ++h)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) o[i][h][j] *= alpha;
+          for (int j = 0; j < VE; ++j) o[i][h][j] *= alpha;
+      }
+      const float base = m[i] == -INFINITY ? 0.f : m[i];  // no finite score yet: all weights are 0
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float x = __builtin_amdgcn_exp2f(s[i][t][r] - base);
-          // 8- and 16-bit caches: the weights enter the product as bf16 (off by half a step, 2^-8 of the weight at
-          // most, as the output's own rounding is), and the sum they are divided by is that of the rounded weights
-          w[i][4 * t + r] = F32 ? x : (float) (__bf16) x;
-          l[i] += w[i][4 * t + r];
-        }
-      if (!F32) {
-        if (DT == MI_DT_E4M3) {
+        for (int r = 0; r < 4; ++r) w[i][4 * t + r] = __builtin_amdgcn_exp2f(s[i][t][r] - base);
+      if constexpr (F32) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+        for (int e = 0; e < 8; ++e) l[i] += w[i][e];
+      } else {
+        // 8- and 16-bit caches: the weights enter the product as bf16 (off by half a step, 2^-8 of the weight at most,
+        // as the output's own rounding is), and the sum they are divided by is that of the rounded weights
+        unsigned int pw[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[i][4 * t + r] *= pow2_bits((f.ev[t] >> (8 * r)) & 255u);
+        for (int e = 0; e < 4; ++e) {
+          pw[e] = pack_bf16(w[i][2 * e], w[i][2 * e + 1]);
+          const float x = __uint_as_float(pw[e] << 16), y = __uint_as_float(pw[e] & 0xffff0000u);
+          l[i] += x;
+          l[i] += y;
+          if constexpr (DT == MI_DT_E4M3)  // times the row's power of two: exact
+            pw[e] = pack_bf16(x * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1))) & 255u),
+                              y * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1) + 8)) & 255u));
         }
-        const uint4 pw = make_uint4(pack_bf16(w[i][0], w[i][1]), pack_bf16(w[i][2], w[i][3]), pack_bf16(w[i][4], w[i][5]),
-                                    pack_bf16(w[i][6], w[i][7]));
-        pf[i] = __builtin_bit_cast(bf8v, pw);
+        pf[i] = __builtin_bit_cast(bf8v, make_uint4(pw[0], pw[1], pw[2], pw[3]));
       }
     }
     if constexpr (F32) {
@@ -652,16 +722,15 @@ __device__ __forceinline__ char* out_row_of(const AttnArgs& p, int64_t b, int he
   return p.out + (b * p.o_seq + (row / p.G) * p.o_tok + (head * p.G + row % p.G) * p.o_head) * QE;
 }
 
-__device__ __forceinline__ int64_t clamped_length(const AttnArgs& p, int64_t b, bool say) {
+__device__ __forceinline__ int64_t clamped_length(const AttnArgs& p, int32_t len, bool say) {
   const int64_t room = (int64_t) p.width << p.page_shift;
-  const int64_t len = p.lengths[b];
   if (len > room && say) report(p.err, MI_IDERR_RANGE);
   return len > room ? room : (len < 0 ? 0 : len);
 }
 
 // Short histories: one wave per (sequence, cache head, tile of 16 query rows).
 template <int DT, int D>
-__global__ __launch_bounds__(256) void hist_attn_short_kernel(AttnArgs p) {
+__global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, 1)) void hist_attn_short_kernel(AttnArgs p) {
   typedef Wave<DT, D, 1> W;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const unsigned int seg = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -670,17 +739,13 @@ __global__ __launch_bounds__(256) void hist_attn_short_kernel(AttnArgs p) {
   const int64_t b = pair / (unsigned int) p.H;
   const int head = (int) (pair - (unsigned int) b * p.H);
   if (b >= p.n_seqs) return;
-  const int64_t len = clamped_length(p, b, lane == 0);
+  const int64_t len = clamped_length(p, scalar_load(p.lengths + b), lane == 0);
   const int row = rt * 16 + c;
   const bool live = row < p.rows;
   W w;
   w.init(0, q_row_of<W::QE>(p, b, head, row, live), live, g);
   const int32_t* table = p.table + b * p.ld_table;
-  for (int64_t pos = 0; pos < len; pos += W::CHUNK) {
-    typename W::Fetched f;
-    W::request(f, p, table, len, pos, head, lane);
-    w.step(f, p, lane);
-  }
+  w.walk(p, table, 0, len, W::CHUNK, head, lane);
   w.close();
   if (live) w.store(0, out_row_of<W::QE>(p, b, head, row), g);
 }
@@ -704,7 +769,7 @@ __device__ __forceinline__ unsigned int units_of(int64_t len) {
 }
 
 template <int DT, int D, int RT>
-__global__ __launch_bounds__(256) void hist_attn_split_kernel(AttnArgs p, SplitArgs a) {
+__global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist_attn_split_kernel(AttnArgs p, SplitArgs a) {
   typedef Wave<DT, D, RT> W;
   __shared__ f4v lo[2][RT * W::VH * W::VE][64];
   __shared__ float2 lml[2][RT][64];
@@ -718,7 +783,7 @@ __global__ __launch_bounds__(256) void hist_attn_split_kernel(AttnArgs p, SplitA
   const unsigned int per = (n_seqs + 255) / 256;
   const unsigned int s0 = threadIdx.x * per, s1 = s0 + per < n_seqs ? s0 + per : n_seqs;
   unsigned int mine = 0;
-  for (unsigned int b = s0; b < s1; ++b) mine += units_of(clamped_length(p, b, blockIdx.x == 0));
+  for (unsigned int b = s0; b < s1; ++b) mine += units_of(clamped_length(p, p.lengths[b], blockIdx.x == 0));
   unsigned int incl = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -741,7 +806,7 @@ __global__ __launch_bounds__(256) void hist_attn_split_kernel(AttnArgs p, SplitA
   if (x0 < total && before * HG <= x0 && x0 < (before + mine) * HG) {
     unsigned int b = s0;
     for (;; ++b) {
-      const unsigned int u = units_of(clamped_length(p, b, false));
+      const unsigned int u = units_of(clamped_length(p, p.lengths[b], false));
       if (x0 < (before + u) * HG) break;
       before += u;
     }
@@ -759,7 +824,7 @@ __global__ __launch_bounds__(256) void hist_attn_split_kernel(AttnArgs p, SplitA
   unsigned int start = __builtin_amdgcn_readfirstlane(found[1]);
   unsigned int x = x0;
   while (x < x1) {
-    const int64_t len = clamped_length(p, b, false);
+    const int64_t len = clamped_length(p, scalar_load(p.lengths + b), false);
     const unsigned int u = units_of(len);
     const unsigned int rem = x - start, pair = rem / u, ub = rem - pair * u;
     const int head = (int) (pair / (unsigned int) a.NG), grp = (int) (pair - (unsigned int) head * a.NG);
@@ -773,13 +838,7 @@ __global__ __launch_bounds__(256) void hist_attn_split_kernel(AttnArgs p, SplitA
     }
     const int32_t* table = p.table + (int64_t) b * p.ld_table;
     const int64_t end = (int64_t) ue * UNIT < len ? (int64_t) ue * UNIT : len;
-    if (row0 < p.rows) {
-      for (int64_t pos = (int64_t) ub * UNIT + ci * W::CHUNK; pos < end; pos += CI * W::CHUNK) {
-        typename W::Fetched f;
-        W::request(f, p, table, len, pos, head, lane);
-        w.step(f, p, lane);
-      }
-    }
+    if (row0 < p.rows) w.walk(p, table, (int64_t) ub * UNIT + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
     w.close();
     // the waves that shared the positions of a row tile: halves fold together, lane by lane
     for (int half = CI >> 1; half > 0; half >>= 1) {
@@ -926,9 +985,6 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void hist_attn_join_kernel(AttnArg
   }
 }
 
-// Workgroups of the split kernel on one CU (a wave on each SIMD): what its registers allow, asked of the compiler.
-constexpr int split_waves(int dim, int RT) { return dim <= 64 ? (RT == 1 ? 4 : 3) : dim == 128 ? 2 : 1; }
-
 // How a call is run; the same on every call of the same sizes.
 struct AttnPlan {
   bool short_rows;
@@ -946,13 +1002,12 @@ AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int
   q.short_rows = room <= 256;
   q.min_run = 1;
   const int64_t most = n_seqs * H * q.NG * mi_cdiv(room, UNIT);
-  const int64_t resident = 256 * split_waves(dim, q.RT);
+  const int64_t resident = 256 * split_waves(dtype == MI_DT_F32, dim, q.RT);
   q.blocks = (int) (most < resident ? most : resident);
   if (!q.short_rows) {
     q.parts_bytes = (size_t) q.blocks * 2 * q.NR * 16 * q.RT * (dim + 4) * sizeof(float);
     q.bytes = q.parts_bytes + (size_t) q.blocks * sizeof(int4);
   }
-  (void) dtype;
   return q;
 }
 
