@@ -312,7 +312,7 @@ int launch_rows(const RowArgs& p, int dim, hipStream_t s) {
 struct AttnArgs {
   const char* kv;
   const uint8_t* exps;
-  int64_t n_pages;
+  int n_pages;
   int H, page_shift;
   const char* q;
   int64_t q_seq, q_tok, q_head;  // strides in elements
@@ -338,7 +338,7 @@ struct AttnArgs {
 // score, probability or value crosses lanes; only the row maximum and sum do (over the four g).
 // Waves on a SIMD, asked of the compiler (registers) and counted on when the work is cut.
 constexpr int split_waves(bool f32, int dim, int RT) {
-  return dim == 256 ? 1 : dim == 128 ? (f32 && RT == 2 ? 1 : 2) : dim == 64 ? (f32 ? 3 : 4) - (RT - 1) : 4 - (RT - 1);
+  return dim == 256 ? 1 : dim == 128 ? (f32 ? 3 - RT : 4 - RT) : dim == 64 ? (f32 ? 3 : 4) - (RT - 1) : 4 - (RT - 1);
 }
 
 template <int DT, int D, int RT>
@@ -412,46 +412,59 @@ struct Wave {
     }
   }
 
-  // A chunk's two tiles: first K row of each in the cache, and how many positions are live (both wave-uniform).
+  // What is known of a chunk ahead of its loads, all of it wave-uniform: the page ids of its two tiles ...
+  struct Ahead {
+    unsigned int first[2];  // position of each tile; a tile behind the end stands where the last one does
+    int valid[2];           // live positions (0: behind the end)
+    int32_t id[2];
+  };
+  // ... and, once those have arrived, the tiles' first K rows in the cache.
   struct Where {
     int64_t rows[2];
     int valid[2];
   };
-  // The 32 positions from `pos` of a history walked up to `len` (table: the sequence's pages).  Tiles behind, or on a bad
-  // page, count as dead and stand at page 0; a chunk that lies behind the end as a whole stands where `last` does.
-  static __device__ __forceinline__ Where locate(const AttnArgs& p, const int32_t* table, int64_t len, int64_t pos, int head,
-                                                 const Where& last, int lane) {
-    Where w = last;
-    w.valid[0] = w.valid[1] = 0;
-    if (pos < len) {
+  static __device__ __forceinline__ Ahead look(const AttnArgs& p, const int32_t* table, unsigned int pos, unsigned int end) {
+    Ahead a;
+    const unsigned int last = (end - 1) & ~15u;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int64_t first = pos + 16 * t;
-        int64_t page = first < len ? scalar_load(table + (first >> p.page_shift)) : 0;
-        w.valid[t] = first >= len ? 0 : (len - first < 16 ? (int) (len - first) : 16);
-        if (page < 0 || page >= p.n_pages) {
-          if (lane == 0) report(p.err, MI_IDERR_RANGE);
-          page = 0;
-          w.valid[t] = 0;
-        }
-        w.rows[t] = (((page * p.H + head) * 2) << p.page_shift) + (first & ((1 << p.page_shift) - 1));
-      }
+    for (int t = 0; t < 2; ++t) {
+      const unsigned int first = pos + 16 * t;
+      a.valid[t] = first >= end ? 0 : (end - first < 16 ? (int) (end - first) : 16);
+      a.first[t] = first < last ? first : last;
+      a.id[t] = scalar_load(table + (a.first[t] >> p.page_shift));
     }
+    return a;
+  }
+  // a tile on a bad page counts as dead and stands on page 0
+  static __device__ __forceinline__ Where locate(const AttnArgs& p, const Ahead& a, int head, int lane) {
+    Where w;
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bool ok = (unsigned int) a.id[t] < (unsigned int) p.n_pages;
+      bad |= !ok && a.valid[t] > 0;
+      const unsigned int page = ok ? (unsigned int) a.id[t] : 0u;
+      w.valid[t] = ok ? a.valid[t] : 0;
+      w.rows[t] = (int64_t) ((((uint64_t) page * (unsigned int) p.H + (unsigned int) head) << (p.page_shift + 1)) +
+                             (a.first[t] & ((1u << p.page_shift) - 1)));
+    }
+    if (bad && lane == 0) report(p.err, MI_IDERR_RANGE);
     return w;
   }
+  // base uniform, 32-bit offset per lane
   static __device__ __forceinline__ void request_k(Fetched& f, const AttnArgs& p, const Where& w, int lane) {
-    const int g = lane >> 4, c = lane & 15;
+    const unsigned int g = lane >> 4, c = lane & 15;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const char* kb = p.kv + w.rows[t] * (D * E);
 #pragma unroll
-      for (int s = 0; s < KL; ++s) fetch<KB>(f.k[t][s], kb + c * (D * E) + s * (KB * 4) + g * KB);
+      for (int s = 0; s < KL; ++s) fetch<KB>(f.k[t][s], kb + s * (KB * 4) + (c * (D * E) + g * KB));
       if (DT == MI_DT_E4M3) f.ek[t] = *reinterpret_cast<const unsigned int*>(p.exps + w.rows[t] + 4 * g);
     }
     __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the work they are to overlap
   }
   static __device__ __forceinline__ void request_v(Fetched& f, const AttnArgs& p, const Where& w, int lane) {
-    const int g = lane >> 4, c = lane & 15;
+    const unsigned int g = lane >> 4, c = lane & 15;
     const int page_size = 1 << p.page_shift;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -460,26 +473,27 @@ struct Wave {
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int h = 0; h < VH; ++h)
-          fetch<VB>(f.v[t][r][h], vb + (4 * g + r) * (D * E) + h * (VB * 16) + c * VB);
+          fetch<VB>(f.v[t][r][h], vb + r * (D * E) + h * (VB * 16) + (4 * g * (D * E) + c * VB));
       if (DT == MI_DT_E4M3) f.ev[t] = *reinterpret_cast<const unsigned int*>(p.exps + w.rows[t] + page_size + 4 * g);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // All chunks pos, pos + stride, ... < end.  A chunk's K is requested while the values of the one before are summed,
-  // its V while its own scores are formed: one set of registers, and loads in flight all the time.  Behind the end the
-  // last chunk is requested again (from the caches): a load that some steps skip would make every step wait for all.
-  __device__ __forceinline__ void walk(const AttnArgs& p, const int32_t* table, int64_t pos, int64_t end, int64_t stride,
-                                       int head, int lane) {
+  // All chunks pos, pos + stride, ... < end.  A chunk's page ids are requested two steps ahead, its K while the values
+  // of the chunk before are summed, its V while its own scores are formed: one set of registers, and loads in flight all
+  // the time.  Behind the end the last chunk is requested again (from the caches): a load that some steps skip would
+  // make every step wait for all loads.
+  __device__ __forceinline__ void walk(const AttnArgs& p, const int32_t* table, unsigned int pos, unsigned int end,
+                                       unsigned int stride, int head, int lane) {
     if (pos >= end) return;
     Fetched f;
-    Where at, next;
-    at.rows[0] = at.rows[1] = 0;
-    at = locate(p, table, end, pos, head, at, lane);
+    Where at = locate(p, look(p, table, pos, end), head, lane);
+    Ahead ahead = look(p, table, pos + stride, end);
     request_k(f, p, at, lane);
     request_v(f, p, at, lane);
     for (;;) {
-      next = locate(p, table, end, pos + stride, head, at, lane);
+      const Where next = locate(p, ahead, head, lane);
+      ahead = look(p, table, pos + 2 * stride, end);
       f4v s[RT][2];
       scores(s, f, p);
       request_k(f, p, next, lane);
@@ -745,7 +759,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, 1)) void hist_
   W w;
   w.init(0, q_row_of<W::QE>(p, b, head, row, live), live, g);
   const int32_t* table = p.table + b * p.ld_table;
-  w.walk(p, table, 0, len, W::CHUNK, head, lane);
+  w.walk(p, table, 0, (unsigned int) len, W::CHUNK, head, lane);
   w.close();
   if (live) w.store(0, out_row_of<W::QE>(p, b, head, row), g);
 }
@@ -837,8 +851,8 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
       w.init(t, q_row_of<W::QE>(p, b, head, row, row < p.rows), row < p.rows, g);
     }
     const int32_t* table = p.table + (int64_t) b * p.ld_table;
-    const int64_t end = (int64_t) ue * UNIT < len ? (int64_t) ue * UNIT : len;
-    if (row0 < p.rows) w.walk(p, table, (int64_t) ub * UNIT + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
+    const unsigned int end = ue == u ? (unsigned int) len : ue * UNIT;
+    if (row0 < p.rows) w.walk(p, table, ub * UNIT + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
     w.close();
     // the waves that shared the positions of a row tile: halves fold together, lane by lane
     for (int half = CI >> 1; half > 0; half >>= 1) {
@@ -1179,7 +1193,7 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
   AttnArgs p = {};
   p.kv = (const char*) cache->kv;
   p.exps = (const uint8_t*) cache->exps;
-  p.n_pages = cache->n_pages;
+  p.n_pages = (int) cache->n_pages;
   p.H = cache->n_heads;
   p.page_shift = log2_of(cache->page_size);
   p.q = (const char*) q;
