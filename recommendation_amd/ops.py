@@ -1032,7 +1032,7 @@ class HistCache(object):
         _need_cuda(kv, exps)
         if exps is not None and exps.device != kv.device:
             raise MiError("HistCache: kv and exps lie on different devices")
-        self.kv, self.exps, self.dtype = kv, exps, dtype
+        self.kv, self.exps, self.dtype, self._index = kv, exps, dtype, kv.get_device()
         self.n_pages, self.n_heads, _, self.page_size, self.dim = shape
         self.c = _lib.HistCacheC(kv=kv.data_ptr(), exps=exps.data_ptr() if exps is not None else None,
                                  n_pages=self.n_pages, n_heads=self.n_heads, page_size=self.page_size, dim=self.dim,
@@ -1043,50 +1043,51 @@ class HistCache(object):
         return self._ref
 
 
-def _hist_common(what, cache, page_table, lengths, offsets, err, *more):
-    """Checks what every history call takes; returns the number of sequences."""
-    _need_cuda(page_table, lengths, offsets, err, *more)
-    dev = cache.kv.device
-    for t in (page_table, lengths, offsets, err) + more:
-        if t is not None and t.device != dev:
-            raise MiError("%s: a tensor lies on %s, the cache on %s" % (what, t.device, dev))
-    if _RAW_DEVICE is not None and dev.index != _RAW_DEVICE():
-        raise MiError("%s: the cache lies on %s, which is not the current device" % (what, dev))
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1 or \
-            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+def _hist_common(what, cache, page_table, lengths, offsets, err, x, y):
+    """Checks what every history call takes; returns (sequences, pages of room, row stride of the table).  These calls
+    are made once per served event: every attribute of a tensor costs ~0.1 us, so each is read once."""
+    dev = cache._index
+    if page_table.get_device() != dev or lengths.get_device() != dev or x.get_device() != dev or \
+            (y is not None and y.get_device() != dev) or (offsets is not None and offsets.get_device() != dev) or \
+            (err is not None and err.get_device() != dev):
+        ts = (page_table, lengths, offsets, err, x, y)
+        _need_cuda(*ts)
+        raise MiError("%s: tensors on %s, the cache on %s" % (what, sorted(set(str(t.device) for t in ts if t is not None)),
+                                                              cache.kv.device))
+    if (_RAW_DEVICE or torch.cuda.current_device)() != dev:
+        raise MiError("%s: the cache lies on %s, which is not the current device" % (what, cache.kv.device))
+    shape, stride = page_table.shape, page_table.stride()
+    if len(shape) != 2 or page_table.dtype is not torch.int32 or shape[1] < 1 or (stride[1] != 1 and shape[1] > 1):
         raise MiError("%s: page_table must be int32 [sequences, pages] with contiguous rows" % what)
-    n = page_table.shape[0]
-    if tuple(lengths.shape) != (n,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+    n = shape[0]
+    if lengths.shape != (n,) or lengths.dtype is not torch.int32 or not lengths.is_contiguous():
         raise MiError("%s: lengths must be contiguous int32 [%d]" % (what, n))
-    if offsets is not None and (tuple(offsets.shape) != (n + 1,) or offsets.dtype != torch.int64 or
-                                not offsets.is_contiguous()):
+    if offsets is not None and (offsets.shape != (n + 1,) or offsets.dtype is not torch.int64 or not offsets.is_contiguous()):
         raise MiError("%s: offsets must be contiguous int64 [%d]" % (what, n + 1))
-    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
+    if err is not None and (err.dtype is not torch.int32 or err.numel() < 1):
         raise MiError("%s: err must be an int32 error word (new_error_word)" % what)
-    return n
-
-
-def _hist_rows(what, cache, x):
-    if x.dim() != 3 or x.shape[1] != cache.n_heads or x.shape[2] != cache.dim:
-        raise MiError("%s: rows must be [n, %d, %d], got %s" % (what, cache.n_heads, cache.dim, tuple(x.shape)))
-    if x.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError("%s: rows must be float32 or bfloat16, got %s" % (what, x.dtype))
-    if x.stride(2) != 1:
-        raise MiError("%s: the values of a row must be contiguous" % what)
-    # a dimension of one entry is never stepped over: its stride says nothing
-    return x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
+    return n, shape[1], stride[0]
 
 
 def _hist_rows_call(name, what, cache, k, v, page_table, lengths, offsets, err):
-    n = _hist_common(what, cache, page_table, lengths, offsets, err, k, v)
-    if k.shape != v.shape or k.dtype != v.dtype:
+    n, width, ld_table = _hist_common(what, cache, page_table, lengths, offsets, err, k, v)
+    shape, dtype = k.shape, k.dtype
+    if shape != v.shape or dtype is not v.dtype:
         raise MiError("%s: k and v differ in shape or type" % what)
-    (k_row, k_head), (v_row, v_head) = _hist_rows(what, cache, k), _hist_rows(what, cache, v)
-    if offsets is None and n and k.shape[0] % n:
-        raise MiError("%s: %d rows do not divide among %d sequences (pass offsets)" % (what, k.shape[0], n))
-    _lib.call(name, cache.ref(), _p(k), _p(v), MI_DT_BF16 if k.dtype == torch.bfloat16 else MI_DT_F32, k_row, k_head, v_row,
-              v_head, k.shape[0], _p(offsets), n, _p(page_table), page_table.stride(0), page_table.shape[1], _p(lengths),
-              _p(err), _stream())
+    if len(shape) != 3 or shape[1] != cache.n_heads or shape[2] != cache.dim:
+        raise MiError("%s: rows must be [n, %d, %d], got %s" % (what, cache.n_heads, cache.dim, tuple(shape)))
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise TypeError("%s: rows must be float32 or bfloat16, got %s" % (what, dtype))
+    ks, vs, rows = k.stride(), v.stride(), shape[0]
+    if ks[2] != 1 or vs[2] != 1:
+        raise MiError("%s: the values of a row must be contiguous" % what)
+    if offsets is None and n and rows % n:
+        raise MiError("%s: %d rows do not divide among %d sequences (pass offsets)" % (what, rows, n))
+    if rows <= 1 or shape[1] == 1:  # a dimension of one entry is never stepped over: its stride says nothing
+        ks, vs = ([0 if shape[d] <= 1 else st[d] for d in range(2)] for st in (ks, vs))
+    _lib.call(name, cache._ref, k.data_ptr(), v.data_ptr(), MI_DT_BF16 if dtype is torch.bfloat16 else MI_DT_F32, ks[0], ks[1],
+              vs[0], vs[1], rows, offsets.data_ptr() if offsets is not None else None, n, page_table.data_ptr(), ld_table,
+              width, lengths.data_ptr(), err.data_ptr() if err is not None else None, _stream())
 
 
 def hist_write(cache, k, v, page_table, lengths, offsets=None, err=None):
@@ -1104,8 +1105,8 @@ def hist_read(cache, page_table, lengths, n_rows=None, offsets=None, dtype=torch
     if out is None:
         if n_rows is None:
             raise MiError("hist_read: give n_rows or out")
-        shape = (int(n_rows), cache.n_heads, cache.dim)
-        out = (torch.empty(shape, dtype=dtype, device=cache.kv.device), torch.empty(shape, dtype=dtype, device=cache.kv.device))
+        k = torch.empty((int(n_rows), cache.n_heads, cache.dim), dtype=dtype, device=cache.kv.device)
+        out = k, torch.empty_like(k)
     elif n_rows is not None and out[0].shape[0] != n_rows:
         raise MiError("hist_read: out holds %d rows, n_rows says %d" % (out[0].shape[0], n_rows))
     k, v = out
@@ -1118,25 +1119,33 @@ def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
     heads, dim] over all ``lengths`` positions of its history; the query heads share the cache's heads in equal groups.
     q: float32 over a float32 cache, bfloat16 otherwise; the result has its shape and type.  ``scale``: of the scores,
     dim ** -0.5 by default.  A sequence without history gives zeros."""
-    n = _hist_common('hist_attn', cache, page_table, lengths, None, err, q, out)
-    q4 = q.unsqueeze(1) if q.dim() == 3 else q
-    if q4.dim() != 4 or q4.shape[0] != n or q4.shape[3] != cache.dim or q4.shape[2] < 1 or q4.shape[2] % cache.n_heads:
-        raise MiError("hist_attn: q must be [%d, (tokens,) a multiple of %d heads, %d], got %s"
-                      % (n, cache.n_heads, cache.dim, tuple(q.shape)))
-    want = torch.float32 if cache.dtype == torch.float32 else torch.bfloat16
-    if q.dtype != want:
-        raise TypeError("hist_attn: q must be %s over a %s cache, got %s" % (want, cache.dtype, q.dtype))
+    n, width, ld_table = _hist_common('hist_attn', cache, page_table, lengths, None, err, q, out)
+    shape, dtype, heads, dim = q.shape, q.dtype, cache.n_heads, cache.dim
+    if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != dim or shape[-2] < 1 or shape[-2] % heads:
+        raise MiError("hist_attn: q must be [%d, (tokens,) a multiple of %d heads, %d], got %s" % (n, heads, dim, tuple(shape)))
+    if dtype is not (torch.float32 if cache.dtype is torch.float32 else torch.bfloat16):
+        raise TypeError("hist_attn: q must be %s over a %s cache, got %s"
+                        % (torch.float32 if cache.dtype is torch.float32 else torch.bfloat16, cache.dtype, dtype))
     if out is None:
-        out = torch.empty(q.shape, dtype=want, device=q.device)
-    elif out.shape != q.shape or out.dtype != want:
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not dtype:
         raise MiError("hist_attn: out must have q's shape and type")
-    o4 = out.unsqueeze(1) if out.dim() == 3 else out
-    if q4.stride(3) != 1 or o4.stride(3) != 1:
+    qs, os_ = q.stride(), out.stride()
+    if qs[-1] != 1 or os_[-1] != 1:
         raise MiError("hist_attn: the values of a row must be contiguous")
-    qs, os_ = ([t.stride(d) if t.shape[d] > 1 else 0 for d in range(3)] for t in (q4, o4))
-    ws_bytes = _lib.load().mi_hist_attn_workspace_bytes(cache.ref(), n, q4.shape[1], q4.shape[2], page_table.shape[1])
+    # sequence, token and head strides; a dimension of one entry is never stepped over: its stride says nothing
+    if len(shape) == 3:
+        tokens = 1
+        qs, os_ = (qs[0], 0, qs[1]), (os_[0], 0, os_[1])
+    else:
+        tokens = shape[1]
+    if n <= 1 or shape[-2] == 1 or tokens == 1:
+        sizes = (n, tokens, shape[-2])
+        qs, os_ = ([st[d] if sizes[d] > 1 else 0 for d in range(3)] for st in (qs, os_))
+    ws_bytes = _lib.load().mi_hist_attn_workspace_bytes(cache._ref, n, tokens, shape[-2], width)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    _lib.call('mi_hist_attn', cache.ref(), _p(q), qs[0], qs[1], qs[2], q4.shape[2], q4.shape[1], n, _p(page_table),
-              page_table.stride(0), page_table.shape[1], _p(lengths), cache.dim ** -0.5 if scale is None else scale, _p(out),
-              os_[0], os_[1], os_[2], _p(ws), ws_bytes, _p(err), _stream())
+    _lib.call('mi_hist_attn', cache._ref, q.data_ptr(), qs[0], qs[1], qs[2], shape[-2], tokens, n, page_table.data_ptr(),
+              ld_table, width, lengths.data_ptr(), dim ** -0.5 if scale is None else scale, out.data_ptr(), os_[0], os_[1],
+              os_[2], ws.data_ptr() if ws is not None else None, ws_bytes, err.data_ptr() if err is not None else None,
+              _stream())
     return out
