@@ -88,12 +88,11 @@ __device__ __forceinline__ int64_t wave_upper_bound(const int64_t* __restrict__ 
   return lo;
 }
 
-// Where row i of the call lives: false if no sequence owns it.  [b0, b1]: the sequences the wave's rows can belong to.
-struct Place {
-  int64_t page;  // -1: the row has no place (in front of position 0, or a bad page)
-  int slot;
-};
-__device__ __forceinline__ bool find_place(const RowArgs& p, int64_t i, int64_t b0, int64_t b1, Place* out) {
+// Where row i of the call lives: index of its K row of head 0 in the cache, or one of the two below.  [b0, b1]: the
+// sequences it can belong to.
+constexpr int64_t NOWHERE = -1;  // in front of position 0, or a bad page
+constexpr int64_t UNOWNED = -2;  // no sequence's row
+__device__ __forceinline__ int64_t find_place(const RowArgs& p, int64_t i, int64_t b0, int64_t b1) {
   int64_t b, last;
   if (p.offsets) {
     while (b0 < b1) {  // the last b with offsets[b] <= i
@@ -101,7 +100,7 @@ __device__ __forceinline__ bool find_place(const RowArgs& p, int64_t i, int64_t 
       if (p.offsets[mid] <= i) b0 = mid; else b1 = mid - 1;
     }
     b = b0;
-    if (b < 0 || b >= p.n_seqs) return false;
+    if (b < 0 || b >= p.n_seqs) return UNOWNED;
     last = p.offsets[b + 1];
   } else {
     b = (int64_t) ((uint32_t) i / (uint32_t) p.each);
@@ -109,43 +108,55 @@ __device__ __forceinline__ bool find_place(const RowArgs& p, int64_t i, int64_t 
   }
   const int64_t len = p.lengths[b];
   const int64_t pos = len - (last - i);
-  out->page = -1;
-  out->slot = 0;
-  if (pos < 0 || pos >= len) return true;
+  if (pos < 0 || pos >= len) return NOWHERE;
   const int64_t pi = pos >> p.page_shift;
-  if (pi >= p.width) {
-    report(p.err, MI_IDERR_RANGE);
-    return true;
-  }
-  const int64_t page = p.table[b * p.ld_table + pi];
+  const int64_t page = pi < p.width ? p.table[b * p.ld_table + pi] : -1;
   if (page < 0 || page >= p.n_pages) {
     report(p.err, MI_IDERR_RANGE);
-    return true;
+    return NOWHERE;
   }
-  out->page = page;
-  out->slot = (int) (pos & ((1 << p.page_shift) - 1));
-  return true;
+  return ((page * p.H * 2) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
 }
 
 struct Eight {
   float x[8];
 };
+// eight values as they lie in memory
 template <int DT>
-__device__ __forceinline__ Eight load8(const char* p);
-template <>
-__device__ __forceinline__ Eight load8<MI_DT_F32>(const char* p) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  return Eight{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-}
-template <>
-__device__ __forceinline__ Eight load8<MI_DT_BF16>(const char* p) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  Eight r;
-  const unsigned int w[4] = {a.x, a.y, a.z, a.w};
+struct Raw8 {
+  unsigned int w[Elem<DT>::BYTES * 2];
+};
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load8(const char* p) {
+  Raw8<DT> r;
+  if constexpr (DT == MI_DT_E4M3) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    r.w[0] = a.x; r.w[1] = a.y;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r.x[2 * i] = __uint_as_float(w[i] << 16);
-    r.x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int i = 0; i < Elem<DT>::BYTES / 2; ++i) {
+      const uint4 a = reinterpret_cast<const uint4*>(p)[i];
+      r.w[4 * i] = a.x; r.w[4 * i + 1] = a.y; r.w[4 * i + 2] = a.z; r.w[4 * i + 3] = a.w;
+    }
+  }
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ Eight widen8(const Raw8<DT>& a) {
+  Eight r;
+#pragma unroll
+  for (int i = 0; i < (DT == MI_DT_F32 ? 8 : 4); ++i) {
+    if constexpr (DT == MI_DT_F32) {
+      r.x[i] = __uint_as_float(a.w[i]);
+    } else if constexpr (DT == MI_DT_BF16) {
+      r.x[2 * i] = __uint_as_float(a.w[i] << 16);
+      r.x[2 * i + 1] = __uint_as_float(a.w[i] & 0xffff0000u);
+    } else {  // exact: 4 significant bits
+      const bf2v c = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a.w[i / 2], 1.0f, true)
+                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a.w[i / 2], 1.0f, false);
+      r.x[2 * i] = (float) c[0];
+      r.x[2 * i + 1] = (float) c[1];
+    }
   }
   return r;
 }
@@ -194,99 +205,107 @@ __device__ __forceinline__ uint2 quantise8(const Eight& e, unsigned int exponent
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
   return make_uint2((unsigned int) lo, (unsigned int) hi);
 }
-__device__ __forceinline__ Eight dequantise8(uint2 c, unsigned int exponent) {
-  const float s = pow2_bits(exponent);
-  Eight r;
-  const unsigned int w[2] = {c.x, c.y};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const bf2v lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.0f, false);  // exact: 4 significant bits
-    const bf2v hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.0f, true);
-    r.x[4 * i + 0] = (float) lo[0] * s;
-    r.x[4 * i + 1] = (float) lo[1] * s;
-    r.x[4 * i + 2] = (float) hi[0] * s;
-    r.x[4 * i + 3] = (float) hi[1] * s;
-  }
-  return r;
-}
-
-// D / 8 lanes per cache row; a row is (token, K or V, head), tokens slowest.  UNROLL rows per lane group are requested
-// together.  READ: the cache is the source, k and v the destination.
-constexpr int ROW_UNROLL = 4;
+// A wave moves `tokens` (a power of two, up to 64) consecutive rows of the call.  Lane i first finds the place of token
+// i: the chain of dependent loads (sequence, length, page) is walked once for all of them.  Then D / 8 lanes move one
+// (token, K or V, head) row, tokens fastest, ROW_BATCH of them requested together.  READ: the cache is the source and
+// k, v the destination.
+constexpr int ROW_BATCH = 4;
 
 template <int CT, int IT, int D, bool READ>
-__global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p) {
-  constexpr int LPR = D / 8, GROUPS = 64 / LPR, PER_WAVE = GROUPS * ROW_UNROLL;
+__global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shift) {
+  constexpr int LPR = D / 8, GROUPS = 64 / LPR;
   constexpr int CE = Elem<CT>::BYTES, IE = Elem<IT>::BYTES;
-  const int lane = threadIdx.x & 63;
-  const unsigned int per_token = 2u * (unsigned int) p.H;
-  const unsigned int total = (unsigned int) p.n_rows * per_token;  // checked on the host
-  const unsigned int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const unsigned int r0 = wave * PER_WAVE;
-  if (r0 >= total) return;
-  const unsigned int r1 = r0 + PER_WAVE - 1 < total ? r0 + PER_WAVE - 1 : total - 1;
+  constexpr int FROM = READ ? CT : IT;
+  const int lane = threadIdx.x & 63, c = lane % LPR;
+  const int64_t wave = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t0 = wave << token_shift;
+  if (t0 >= p.n_rows) return;
+  const int n_tok = p.n_rows - t0 < (1 << token_shift) ? (int) (p.n_rows - t0) : 1 << token_shift;
+  const int n_move = (2 * p.H) << token_shift;  // rows to move, those of tokens >= n_tok among them
+
+  struct Row {
+    bool live;
+    int token, part, head;
+  };
+  auto row_of = [&](int i) {
+    const int r = i * GROUPS + lane / LPR;
+    Row x;
+    x.token = r & ((1 << token_shift) - 1);
+    const int hp = r >> token_shift;
+    x.live = r < n_move && x.token < n_tok;
+    x.part = hp >= p.H ? 1 : 0;
+    x.head = hp - x.part * p.H;
+    return x;
+  };
+  auto io = [&](const Row& x) {
+    return const_cast<char*>(x.part ? p.v + ((t0 + x.token) * p.v_row + x.head * p.v_head + c * 8) * IE
+                                    : p.k + ((t0 + x.token) * p.k_row + x.head * p.k_head + c * 8) * IE);
+  };
+  Raw8<FROM> raw[ROW_BATCH];
+  auto load_inputs = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < ROW_BATCH; ++u) {
+      const Row x = row_of(i0 + u);
+      if (x.live) raw[u] = load8<FROM>(io(x));
+      else raw[u] = Raw8<FROM>{};
+    }
+  };
+  if (!READ) load_inputs(0);  // they depend on nothing
+
   int64_t b0 = 0, b1 = 0;
   if (p.offsets) {
-    b0 = wave_upper_bound(p.offsets, p.n_seqs + 1, r0 / per_token, lane) - 1;
-    b1 = wave_upper_bound(p.offsets, p.n_seqs + 1, r1 / per_token, lane) - 1;
+    b0 = wave_upper_bound(p.offsets, p.n_seqs + 1, t0, lane) - 1;
+    b1 = n_tok > 1 ? wave_upper_bound(p.offsets, p.n_seqs + 1, t0 + n_tok - 1, lane) - 1 : b0;
   }
-  const int c = lane % LPR;
-  int64_t tok[ROW_UNROLL];
-  int part[ROW_UNROLL], head[ROW_UNROLL];
-  bool live[ROW_UNROLL];
-  Place at[ROW_UNROLL];
-  Eight x[ROW_UNROLL];
+  // lanes without a token repeat the last one's search
+  const int64_t mine = find_place(p, t0 + (lane < n_tok ? lane : n_tok - 1), b0, b1);
+
+  const int n_iter = (n_move + GROUPS - 1) / GROUPS;
+  for (int i0 = 0; i0 < n_iter; i0 += ROW_BATCH) {
+    int64_t at[ROW_BATCH];
+    unsigned int exponent[ROW_BATCH];
+    if (!READ && i0) load_inputs(i0);
 #pragma unroll
-  for (int u = 0; u < ROW_UNROLL; ++u) {
-    const unsigned int r = r0 + u * GROUPS + lane / LPR;
-    live[u] = r < total;
-    const unsigned int rr = live[u] ? r : r0;
-    tok[u] = rr / per_token;
-    const unsigned int rem = rr - (unsigned int) tok[u] * per_token;
-    part[u] = rem >= (unsigned int) p.H ? 1 : 0;
-    head[u] = (int) rem - part[u] * p.H;
-    if (!READ) {
-      const char* src = part[u] ? p.v + (tok[u] * p.v_row + head[u] * p.v_head + c * 8) * IE
-                                : p.k + (tok[u] * p.k_row + head[u] * p.k_head + c * 8) * IE;
-      x[u] = load8<IT>(src);
+    for (int u = 0; u < ROW_BATCH; ++u) {
+      const Row x = row_of(i0 + u);
+      const int64_t base = __shfl(mine, x.token, 64);
+      at[u] = !x.live ? UNOWNED : base < 0 ? base : base + ((int64_t) (x.head * 2 + x.part) << p.page_shift);
+      exponent[u] = 0;
+      if (READ) {
+        raw[u] = Raw8<FROM>{};
+        if (at[u] >= 0) {
+          raw[u] = load8<FROM>(p.kv + (at[u] * D + c * 8) * CE);
+          if (CT == MI_DT_E4M3) exponent[u] = p.exps[at[u]];
+        }
+      }
     }
-  }
 #pragma unroll
-  for (int u = 0; u < ROW_UNROLL; ++u) {
-    // lanes past the end repeat the wave's first row, which must not be reported twice: harmless, the bit is the same
-    live[u] &= find_place(p, tok[u], b0, b1, &at[u]);
-  }
-#pragma unroll
-  for (int u = 0; u < ROW_UNROLL; ++u) {
-    const int64_t row = (((at[u].page * p.H + head[u]) * 2 + part[u]) << p.page_shift) + at[u].slot;
-    if (READ) {
-      Eight y = Eight{{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
-      if (live[u] && at[u].page >= 0) {
-        const char* src = p.kv + (row * D + c * 8) * CE;
-        if (CT == MI_DT_E4M3) y = dequantise8(*reinterpret_cast<const uint2*>(src), p.exps[row]);
-        else y = load8<CT == MI_DT_E4M3 ? MI_DT_F32 : CT>(src);
-      }
-      if (live[u]) {
-        char* dst = const_cast<char*>(part[u] ? p.v + (tok[u] * p.v_row + head[u] * p.v_head + c * 8) * IE
-                                              : p.k + (tok[u] * p.k_row + head[u] * p.k_head + c * 8) * IE);
-        store8<IT>(dst, y);
-      }
-    } else {
-      float top = 0.f;
-      if (CT == MI_DT_E4M3) {  // all lanes take part in the exchange
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(x[u].x[i]));
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-      }
-      if (live[u] && at[u].page >= 0) {
-        char* dst = p.kv + (row * D + c * 8) * CE;
+    for (int u = 0; u < ROW_BATCH; ++u) {
+      Eight y = widen8<FROM>(raw[u]);
+      if constexpr (READ) {
         if (CT == MI_DT_E4M3) {
-          const unsigned int e = row_exponent(top);
-          *reinterpret_cast<uint2*>(dst) = quantise8(x[u], e);
-          if (c == 0) p.exps[row] = (uint8_t) e;
-        } else {
-          store8<CT == MI_DT_E4M3 ? MI_DT_F32 : CT>(dst, x[u]);
+          const float s = pow2_bits(exponent[u]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y.x[e] *= s;
+        }
+        if (at[u] != UNOWNED) store8<IT>(io(row_of(i0 + u)), y);
+      } else {
+        float top = 0.f;
+        if (CT == MI_DT_E4M3) {  // every lane takes part in the exchange
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, finite_abs(y.x[e]));
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        }
+        if (at[u] >= 0) {
+          char* dst = p.kv + (at[u] * D + c * 8) * CE;
+          if constexpr (CT == MI_DT_E4M3) {
+            const unsigned int e = row_exponent(top);
+            *reinterpret_cast<uint2*>(dst) = quantise8(y, e);
+            if (c == 0) p.exps[at[u]] = (uint8_t) e;
+          } else {
+            store8<CT>(dst, y);
+          }
         }
       }
     }
@@ -295,14 +314,17 @@ __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p) {
 
 template <int CT, int IT, bool READ>
 int launch_rows(const RowArgs& p, int dim, hipStream_t s) {
-  const int64_t rows = p.n_rows * 2 * p.H;
-  const int per_block = 4 * (64 / (dim / 8)) * ROW_UNROLL;
-  const dim3 grid((unsigned int) mi_cdiv(rows, per_block));
+  // at least the rows of one instruction; beyond that, more tokens a wave as long as there are four waves for every SIMD
+  const int groups = 64 / (dim / 8);
+  int shift = 0;
+  while ((2 * p.H) << shift < groups && shift < 6) ++shift;
+  while (shift < 5 && (p.n_rows >> (shift + 1)) >= 4096) ++shift;
+  const dim3 grid((unsigned int) mi_cdiv(p.n_rows, 4ll << shift));
   switch (dim) {
-    case 32: hist_rows_kernel<CT, IT, 32, READ><<<grid, 256, 0, s>>>(p); break;
-    case 64: hist_rows_kernel<CT, IT, 64, READ><<<grid, 256, 0, s>>>(p); break;
-    case 128: hist_rows_kernel<CT, IT, 128, READ><<<grid, 256, 0, s>>>(p); break;
-    default: hist_rows_kernel<CT, IT, 256, READ><<<grid, 256, 0, s>>>(p); break;
+    case 32: hist_rows_kernel<CT, IT, 32, READ><<<grid, 256, 0, s>>>(p, shift); break;
+    case 64: hist_rows_kernel<CT, IT, 64, READ><<<grid, 256, 0, s>>>(p, shift); break;
+    case 128: hist_rows_kernel<CT, IT, 128, READ><<<grid, 256, 0, s>>>(p, shift); break;
+    default: hist_rows_kernel<CT, IT, 256, READ><<<grid, 256, 0, s>>>(p, shift); break;
   }
   MI_LAUNCH_CHECK();
   return MI_OK;
