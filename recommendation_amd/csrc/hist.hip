@@ -14,6 +14,8 @@ namespace {
 typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
+typedef unsigned int u4v __attribute__((ext_vector_type(4)));
+typedef unsigned int u2v __attribute__((ext_vector_type(2)));
 
 template <int DT>
 struct Elem;
@@ -43,6 +45,20 @@ __device__ __forceinline__ float max_over_g(float x) {
 template <typename T>
 __device__ __forceinline__ T scalar_load(const T* p) {
   return *(const __attribute__((address_space(4))) T*) (p);
+}
+
+// Loads and stores past the caches (STREAM) or through them.  More than the last-level cache holds gains from going past
+// it, less loses what an earlier launch left there (measured at each launch below).
+constexpr int64_t LAST_LEVEL_BYTES = 256ll << 20;
+template <bool STREAM, typename T>
+__device__ __forceinline__ T load_of(const T* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool STREAM, typename T>
+__device__ __forceinline__ void store_of(T* p, T x) {
+  if constexpr (STREAM) __builtin_nontemporal_store(x, p);
+  else *p = x;
 }
 
 __device__ __forceinline__ float pow2_bits(unsigned int e) { return __uint_as_float(e << 23); }
@@ -121,25 +137,59 @@ __device__ __forceinline__ int64_t find_place(const RowArgs& p, int64_t i, int64
 struct Eight {
   float x[8];
 };
-// eight values as they lie in memory
+// Eight values of a row as they lie in memory.  A lane's eight are channels 8c .. 8c+7, or with SPLIT 4c .. 4c+3 of each
+// half of the row: where a side holds f32, 16 bytes a lane then make whole lines of a row with every instruction.
 template <int DT>
 struct Raw8 {
   unsigned int w[Elem<DT>::BYTES * 2];
 };
-template <int DT>
-__device__ __forceinline__ Raw8<DT> load8(const char* p) {
-  Raw8<DT> r;
-  if constexpr (DT == MI_DT_E4M3) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    r.w[0] = a.x; r.w[1] = a.y;
-  } else {
+template <int WORDS, bool STREAM>
+__device__ __forceinline__ void load_words(unsigned int* w, const char* p) {
+  if constexpr (WORDS >= 4) {
 #pragma unroll
-    for (int i = 0; i < Elem<DT>::BYTES / 2; ++i) {
-      const uint4 a = reinterpret_cast<const uint4*>(p)[i];
-      r.w[4 * i] = a.x; r.w[4 * i + 1] = a.y; r.w[4 * i + 2] = a.z; r.w[4 * i + 3] = a.w;
+    for (int i = 0; i < WORDS; i += 4) {
+      const u4v a = load_of<STREAM>(reinterpret_cast<const u4v*>(p) + i / 4);
+      w[i] = a[0]; w[i + 1] = a[1]; w[i + 2] = a[2]; w[i + 3] = a[3];
     }
+  } else if constexpr (WORDS == 2) {
+    const u2v a = load_of<STREAM>(reinterpret_cast<const u2v*>(p));
+    w[0] = a[0]; w[1] = a[1];
+  } else {
+    w[0] = load_of<STREAM>(reinterpret_cast<const unsigned int*>(p));
+  }
+}
+template <int WORDS, bool STREAM>
+__device__ __forceinline__ void store_words(char* p, const unsigned int* w) {
+  if constexpr (WORDS >= 4) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) store_of<STREAM>(reinterpret_cast<u4v*>(p) + i / 4, u4v{w[i], w[i + 1], w[i + 2], w[i + 3]});
+  } else if constexpr (WORDS == 2) {
+    store_of<STREAM>(reinterpret_cast<u2v*>(p), u2v{w[0], w[1]});
+  } else {
+    store_of<STREAM>(reinterpret_cast<unsigned int*>(p), w[0]);
+  }
+}
+template <int DT, int D, bool SPLIT, bool STREAM>
+__device__ __forceinline__ Raw8<DT> load8(const char* row, int c) {
+  constexpr int E = Elem<DT>::BYTES;
+  Raw8<DT> r;
+  if constexpr (SPLIT) {
+    load_words<E, STREAM>(r.w, row + c * 4 * E);
+    load_words<E, STREAM>(r.w + E, row + (D / 2 + c * 4) * E);
+  } else {
+    load_words<2 * E, STREAM>(r.w, row + c * 8 * E);
   }
   return r;
+}
+template <int DT, int D, bool SPLIT, bool STREAM>
+__device__ __forceinline__ void store8(char* row, int c, const Raw8<DT>& r) {
+  constexpr int E = Elem<DT>::BYTES;
+  if constexpr (SPLIT) {
+    store_words<E, STREAM>(row + c * 4 * E, r.w);
+    store_words<E, STREAM>(row + (D / 2 + c * 4) * E, r.w + E);
+  } else {
+    store_words<2 * E, STREAM>(row + c * 8 * E, r.w);
+  }
 }
 template <int DT>
 __device__ __forceinline__ Eight widen8(const Raw8<DT>& a) {
@@ -167,16 +217,12 @@ __device__ __forceinline__ unsigned int pack_bf16(float a, float b) {
   return __builtin_bit_cast(unsigned int, p);
 }
 template <int DT>
-__device__ __forceinline__ void store8(char* p, const Eight& e);
-template <>
-__device__ __forceinline__ void store8<MI_DT_F32>(char* p, const Eight& e) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(e.x[0], e.x[1], e.x[2], e.x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(e.x[4], e.x[5], e.x[6], e.x[7]);
-}
-template <>
-__device__ __forceinline__ void store8<MI_DT_BF16>(char* p, const Eight& e) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(e.x[0], e.x[1]), pack_bf16(e.x[2], e.x[3]),
-                                            pack_bf16(e.x[4], e.x[5]), pack_bf16(e.x[6], e.x[7]));
+__device__ __forceinline__ Raw8<DT> round8(const Eight& e) {  // f32, bf16
+  Raw8<DT> r;
+#pragma unroll
+  for (int i = 0; i < Elem<DT>::BYTES * 2; ++i)
+    r.w[i] = DT == MI_DT_F32 ? __float_as_uint(e.x[i]) : pack_bf16(e.x[(2 * i) & 7], e.x[(2 * i + 1) & 7]);
+  return r;
 }
 
 // Quantisation of a row x: a = max finite |x|, e the smallest exponent with a * 2^-e <= 448 (the largest e4m3 value),
@@ -191,7 +237,7 @@ __device__ __forceinline__ unsigned int row_exponent(float top) {  // e + 127
   int biased = (int) (u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);  // top <= 1.75 * 2^k fits 448 * 2^(k-8)
   return biased < 1 ? 1u : (unsigned int) biased;
 }
-__device__ __forceinline__ uint2 quantise8(const Eight& e, unsigned int exponent) {
+__device__ __forceinline__ Raw8<MI_DT_E4M3> quantise8(const Eight& e, unsigned int exponent) {
   const float inv = pow2_bits(254u - exponent);
   float y[8];
 #pragma unroll
@@ -203,7 +249,7 @@ __device__ __forceinline__ uint2 quantise8(const Eight& e, unsigned int exponent
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
   int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
-  return make_uint2((unsigned int) lo, (unsigned int) hi);
+  return Raw8<MI_DT_E4M3>{{(unsigned int) lo, (unsigned int) hi}};
 }
 // A wave moves `tokens` (a power of two, up to 64) consecutive rows of the call.  Lane i first finds the place of token
 // i: the chain of dependent loads (sequence, length, page) is walked once for all of them.  Then D / 8 lanes move one
@@ -211,11 +257,12 @@ __device__ __forceinline__ uint2 quantise8(const Eight& e, unsigned int exponent
 // k, v the destination.
 constexpr int ROW_BATCH = 4;
 
-template <int CT, int IT, int D, bool READ>
+template <int CT, int IT, int D, bool READ, bool STREAM>
 __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shift) {
   constexpr int LPR = D / 8, GROUPS = 64 / LPR;
   constexpr int CE = Elem<CT>::BYTES, IE = Elem<IT>::BYTES;
   constexpr int FROM = READ ? CT : IT;
+  constexpr bool SPLIT = CT == MI_DT_F32 || IT == MI_DT_F32;
   const int lane = threadIdx.x & 63, c = lane % LPR;
   const int64_t wave = (int64_t) blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t0 = wave << token_shift;
@@ -238,15 +285,15 @@ __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shi
     return x;
   };
   auto io = [&](const Row& x) {
-    return const_cast<char*>(x.part ? p.v + ((t0 + x.token) * p.v_row + x.head * p.v_head + c * 8) * IE
-                                    : p.k + ((t0 + x.token) * p.k_row + x.head * p.k_head + c * 8) * IE);
+    return const_cast<char*>(x.part ? p.v + ((t0 + x.token) * p.v_row + x.head * p.v_head) * IE
+                                    : p.k + ((t0 + x.token) * p.k_row + x.head * p.k_head) * IE);
   };
   Raw8<FROM> raw[ROW_BATCH];
   auto load_inputs = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < ROW_BATCH; ++u) {
       const Row x = row_of(i0 + u);
-      if (x.live) raw[u] = load8<FROM>(io(x));
+      if (x.live) raw[u] = load8<FROM, D, SPLIT, STREAM>(io(x), c);
       else raw[u] = Raw8<FROM>{};
     }
   };
@@ -274,7 +321,7 @@ __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shi
       if (READ) {
         raw[u] = Raw8<FROM>{};
         if (at[u] >= 0) {
-          raw[u] = load8<FROM>(p.kv + (at[u] * D + c * 8) * CE);
+          raw[u] = load8<FROM, D, SPLIT, STREAM>(p.kv + at[u] * D * CE, c);
           if (CT == MI_DT_E4M3) exponent[u] = p.exps[at[u]];
         }
       }
@@ -288,7 +335,7 @@ __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shi
 #pragma unroll
           for (int e = 0; e < 8; ++e) y.x[e] *= s;
         }
-        if (at[u] != UNOWNED) store8<IT>(io(row_of(i0 + u)), y);
+        if (at[u] != UNOWNED) store8<IT, D, SPLIT, STREAM>(io(row_of(i0 + u)), c, round8<IT>(y));
       } else {
         float top = 0.f;
         if (CT == MI_DT_E4M3) {  // every lane takes part in the exchange
@@ -298,13 +345,13 @@ __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shi
           for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
         }
         if (at[u] >= 0) {
-          char* dst = p.kv + (at[u] * D + c * 8) * CE;
+          char* dst = p.kv + at[u] * D * CE;
           if constexpr (CT == MI_DT_E4M3) {
             const unsigned int e = row_exponent(top);
-            *reinterpret_cast<uint2*>(dst) = quantise8(y, e);
+            store8<CT, D, SPLIT, false>(dst, c, quantise8(y, e));
             if (c == 0) p.exps[at[u]] = (uint8_t) e;
           } else {
-            store8<CT>(dst, y);
+            store8<CT, D, SPLIT, false>(dst, c, round8<CT>(y));
           }
         }
       }
@@ -318,14 +365,19 @@ int launch_rows(const RowArgs& p, int dim, hipStream_t s) {
   const int groups = 64 / (dim / 8);
   int shift = 0;
   while ((2 * p.H) << shift < groups && shift < 6) ++shift;
-  while (shift < 5 && (p.n_rows >> (shift + 1)) >= 4096) ++shift;
+  while (shift < 2 && (p.n_rows >> (shift + 1)) >= 4096) ++shift;
   const dim3 grid((unsigned int) mi_cdiv(p.n_rows, 4ll << shift));
+  const bool stream = p.n_rows * 2 * p.H * dim * (Elem<CT>::BYTES + Elem<IT>::BYTES) > LAST_LEVEL_BYTES;
+#define MI_HIST_ROWS(D)                                                                            \
+  if (stream) hist_rows_kernel<CT, IT, D, READ, true><<<grid, 256, 0, s>>>(p, shift);              \
+  else hist_rows_kernel<CT, IT, D, READ, false><<<grid, 256, 0, s>>>(p, shift)
   switch (dim) {
-    case 32: hist_rows_kernel<CT, IT, 32, READ><<<grid, 256, 0, s>>>(p, shift); break;
-    case 64: hist_rows_kernel<CT, IT, 64, READ><<<grid, 256, 0, s>>>(p, shift); break;
-    case 128: hist_rows_kernel<CT, IT, 128, READ><<<grid, 256, 0, s>>>(p, shift); break;
-    default: hist_rows_kernel<CT, IT, 256, READ><<<grid, 256, 0, s>>>(p, shift); break;
+    case 32: MI_HIST_ROWS(32); break;
+    case 64: MI_HIST_ROWS(64); break;
+    case 128: MI_HIST_ROWS(128); break;
+    default: MI_HIST_ROWS(256); break;
   }
+#undef MI_HIST_ROWS
   MI_LAUNCH_CHECK();
   return MI_OK;
 }
@@ -363,7 +415,7 @@ constexpr int split_waves(bool f32, int dim, int RT) {
   return dim == 256 ? 1 : dim == 128 ? (f32 ? 3 - RT : 4 - RT) : dim == 64 ? (f32 ? 3 : 4) - (RT - 1) : 4 - (RT - 1);
 }
 
-template <int DT, int D, int RT>
+template <int DT, int D, int RT, bool STREAM>
 struct Wave {
   static constexpr bool F32 = DT == MI_DT_F32;
   static constexpr int E = Elem<DT>::BYTES;
@@ -422,15 +474,15 @@ struct Wave {
   template <int BYTES>
   static __device__ __forceinline__ void fetch(unsigned int* dst, const char* src) {
     if constexpr (BYTES == 16) {
-      const uint4 x = *reinterpret_cast<const uint4*>(src);
-      dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w;
+      const u4v x = load_of<STREAM>(reinterpret_cast<const u4v*>(src));
+      dst[0] = x[0]; dst[1] = x[1]; dst[2] = x[2]; dst[3] = x[3];
     } else if constexpr (BYTES == 8) {
-      const uint2 x = *reinterpret_cast<const uint2*>(src);
-      dst[0] = x.x; dst[1] = x.y;
+      const u2v x = load_of<STREAM>(reinterpret_cast<const u2v*>(src));
+      dst[0] = x[0]; dst[1] = x[1];
     } else if constexpr (BYTES == 4) {
-      dst[0] = *reinterpret_cast<const unsigned int*>(src);
+      dst[0] = load_of<STREAM>(reinterpret_cast<const unsigned int*>(src));
     } else {
-      dst[0] = *reinterpret_cast<const unsigned short*>(src);
+      dst[0] = load_of<STREAM>(reinterpret_cast<const unsigned short*>(src));
     }
   }
 
@@ -765,9 +817,9 @@ __device__ __forceinline__ int64_t clamped_length(const AttnArgs& p, int32_t len
 }
 
 // Short histories: one wave per (sequence, cache head, tile of 16 query rows).
-template <int DT, int D>
+template <int DT, int D, bool STREAM>
 __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, 1)) void hist_attn_short_kernel(AttnArgs p) {
-  typedef Wave<DT, D, 1> W;
+  typedef Wave<DT, D, 1, STREAM> W;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const unsigned int seg = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned int pair = seg / (unsigned int) p.n_rt;
@@ -804,9 +856,9 @@ __device__ __forceinline__ unsigned int units_of(int64_t len) {
   return len <= UNIT ? 1u : (unsigned int) ((len + UNIT - 1) / UNIT);
 }
 
-template <int DT, int D, int RT>
+template <int DT, int D, int RT, bool STREAM>
 __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist_attn_split_kernel(AttnArgs p, SplitArgs a) {
-  typedef Wave<DT, D, RT> W;
+  typedef Wave<DT, D, RT, STREAM> W;
   __shared__ f4v lo[2][RT * W::VH * W::VE][64];
   __shared__ float2 lml[2][RT][64];
   __shared__ unsigned int wave_sum[4];
@@ -1047,10 +1099,10 @@ AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int
   return q;
 }
 
-template <int DT, int D>
+template <int DT, int D, bool STREAM>
 int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) {
   if (q.short_rows) {
-    hist_attn_short_kernel<DT, D><<<dim3((unsigned int) mi_cdiv(p.n_seqs * p.H * p.n_rt, 4)), 256, 0, s>>>(p);
+    hist_attn_short_kernel<DT, D, STREAM><<<dim3((unsigned int) mi_cdiv(p.n_seqs * p.H * p.n_rt, 4)), 256, 0, s>>>(p);
     MI_LAUNCH_CHECK();
     return MI_OK;
   }
@@ -1060,8 +1112,8 @@ int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t 
   a.min_run = q.min_run;
   a.parts = (float*) ws;
   a.meta = (int4*) ((char*) ws + q.parts_bytes);
-  if (q.RT == 2) hist_attn_split_kernel<DT, D, D <= 128 ? 2 : 1><<<q.blocks, 256, 0, s>>>(p, a);
-  else hist_attn_split_kernel<DT, D, 1><<<q.blocks, 256, 0, s>>>(p, a);
+  if (q.RT == 2) hist_attn_split_kernel<DT, D, D <= 128 ? 2 : 1, STREAM><<<q.blocks, 256, 0, s>>>(p, a);
+  else hist_attn_split_kernel<DT, D, 1, STREAM><<<q.blocks, 256, 0, s>>>(p, a);
   MI_LAUNCH_CHECK();
   const int group_rows = q.NR * 16 * q.RT;
   const dim3 grid(q.blocks, (unsigned int) mi_cdiv(p.rows < group_rows ? p.rows : group_rows, JOIN_WAVES));
@@ -1072,11 +1124,12 @@ int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t 
 
 template <int DT>
 int launch_attn(const AttnArgs& p, const AttnPlan& q, int dim, void* ws, hipStream_t s) {
+  const bool stream = ((int64_t) p.n_pages * p.H * 2 << p.page_shift) * dim * Elem<DT>::BYTES > LAST_LEVEL_BYTES;
   switch (dim) {
-    case 32: return launch_attn_dim<DT, 32>(p, q, ws, s);
-    case 64: return launch_attn_dim<DT, 64>(p, q, ws, s);
-    case 128: return launch_attn_dim<DT, 128>(p, q, ws, s);
-    default: return launch_attn_dim<DT, 256>(p, q, ws, s);
+    case 32: return stream ? launch_attn_dim<DT, 32, true>(p, q, ws, s) : launch_attn_dim<DT, 32, false>(p, q, ws, s);
+    case 64: return stream ? launch_attn_dim<DT, 64, true>(p, q, ws, s) : launch_attn_dim<DT, 64, false>(p, q, ws, s);
+    case 128: return stream ? launch_attn_dim<DT, 128, true>(p, q, ws, s) : launch_attn_dim<DT, 128, false>(p, q, ws, s);
+    default: return stream ? launch_attn_dim<DT, 256, true>(p, q, ws, s) : launch_attn_dim<DT, 256, false>(p, q, ws, s);
   }
 }
 
