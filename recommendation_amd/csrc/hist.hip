@@ -433,7 +433,9 @@ struct Wave {
   static constexpr float SLACK = 8.f;
 
   f4v o[RT][VH][VE];
-  float m[RT], l[RT];
+  // l: a column of the second product whose "values" are all 1, so that every lane of a row holds the whole sum
+  float m[RT];
+  f4v l[RT];
   bf8v qf[RT][F32 ? 1 : NS];
   f4v qv[RT][F32 ? KL : 1];
 
@@ -445,7 +447,7 @@ struct Wave {
 
   __device__ __forceinline__ void init(int t, const char* q_row, bool live, int g) {
     m[t] = -INFINITY;
-    l[t] = 0.f;
+    l[t] = f4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < VH; ++h)
 #pragma unroll
@@ -623,12 +625,10 @@ struct Wave {
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
+        // (scale first: a small power of two times it could leave the normal range)
         const float e = DT == MI_DT_E4M3 ? pow2_bits((f.ek[t] >> (8 * r)) & 255u) : 1.f;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          s[i][t][r] *= p.scale;
-          if (DT == MI_DT_E4M3) s[i][t][r] *= e;
-        }
+        for (int i = 0; i < RT; ++i) s[i][t][r] = DT == MI_DT_E4M3 ? s[i][t][r] * p.scale * e : s[i][t][r] * p.scale;
       }
     }
   }
@@ -653,6 +653,15 @@ struct Wave {
     }
     float w[RT][8];
     bf8v pf[RT];
+    uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);  // bf16
+    if constexpr (DT == MI_DT_E4M3) {
+      unsigned int* po = &ones.x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // exponent field 254 - exps; dead positions (0 here) have weight 0
+        const unsigned int two = f.ev[e >> 1] >> (16 * (e & 1));
+        po[e] = 0x7f007f00u - (((two & 255u) << 7) | ((two & 0xff00u) << 15));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       float top = m[i];
@@ -678,24 +687,24 @@ struct Wave {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[i][4 * t + r] = __builtin_amdgcn_exp2f(s[i][t][r] - base);
+      // 8- and 16-bit caches: the weights enter the product as bf16 (off by half a step, 2^-8 of the weight at most, as
+      // the output's own rounding is), and the sum they are divided by is that of the rounded weights.  In 8 bits they
+      // are multiplied by the value row's power of two, exactly, and their sum's column holds its inverse.
       if constexpr (F32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) l[i] += w[i][e];
+        for (int e = 0; e < 8; ++e) l[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.f, w[i][e], l[i], 0, 0, 0);
       } else {
-        // 8- and 16-bit caches: the weights enter the product as bf16 (off by half a step, 2^-8 of the weight at most,
-        // as the output's own rounding is), and the sum they are divided by is that of the rounded weights
         unsigned int pw[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pw[e] = pack_bf16(w[i][2 * e], w[i][2 * e + 1]);
-          const float x = __uint_as_float(pw[e] << 16), y = __uint_as_float(pw[e] & 0xffff0000u);
-          l[i] += x;
-          l[i] += y;
-          if constexpr (DT == MI_DT_E4M3)  // times the row's power of two: exact
-            pw[e] = pack_bf16(x * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1))) & 255u),
-                              y * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1) + 8)) & 255u));
+          if constexpr (DT == MI_DT_E4M3)
+            pw[e] = pack_bf16(w[i][2 * e] * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1))) & 255u),
+                              w[i][2 * e + 1] * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1) + 8)) & 255u));
+          else
+            pw[e] = pack_bf16(w[i][2 * e], w[i][2 * e + 1]);
         }
         pf[i] = __builtin_bit_cast(bf8v, make_uint4(pw[0], pw[1], pw[2], pw[3]));
+        l[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, ones), pf[i], l[i], 0, 0, 0);
       }
     }
     if constexpr (F32) {
@@ -742,18 +751,9 @@ struct Wave {
     }
   }
 
-  // row sums over the four g (every lane of a row ends with the same l)
-  __device__ __forceinline__ void close() {
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      l[i] += __shfl_xor(l[i], 16, 64);
-      l[i] += __shfl_xor(l[i], 32, 64);
-    }
-  }
-
   // lane (g, c) holds channels h * (D / VH) + (4 g + r) * VE + j of query row c: contiguous in (r, j)
   __device__ __forceinline__ void store(int t, char* out_row, int g) {
-    const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
+    const float inv = l[t][0] == 0.f ? 0.f : 1.f / l[t][0];
 #pragma unroll
     for (int h = 0; h < VH; ++h) {
       char* dst = out_row + (h * (D / VH) + 4 * g * VE) * QE;
@@ -775,18 +775,18 @@ struct Wave {
     }
   }
 
-  // unnormalised, in f32, for the joining launch: [D] sums, then m and l
-  __device__ __forceinline__ void store_part(int t, float* part_row, int g) {
+  // unnormalised, in f32, for the joining launch: a row's D sums as the registers hold them (channel_of), and m, l
+  __device__ __forceinline__ void store_part(int t, float* part_row, float2* ml, int g) {
 #pragma unroll
-    for (int h = 0; h < VH; ++h) {
-      float* dst = part_row + h * (D / VH) + 4 * g * VE;
+    for (int h = 0; h < VH; ++h)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < VE; j += 2)
-          *reinterpret_cast<float2*>(dst + r * VE + j) = make_float2(o[t][h][j][r], o[t][h][j + 1][r]);
-    }
-    if (g == 0) *reinterpret_cast<float2*>(part_row + D) = make_float2(m[t], l[t]);
+      for (int j = 0; j < VE; ++j) *reinterpret_cast<f4v*>(part_row + (h * VE + j) * 16 + g * 4) = o[t][h][j];
+    if (g == 0) *ml = make_float2(m[t], l[t][0]);
+  }
+  // channel of element r of the 16-byte piece `piece` of such a row
+  static __device__ __forceinline__ int channel_of(int piece, int r) {
+    const int i = piece >> 2, g = piece & 3;
+    return (i / VE) * (D / VH) + (4 * g + r) * VE + i % VE;
   }
 };
 
@@ -834,7 +834,6 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, 1)) void hist_
   w.init(0, q_row_of<W::QE>(p, b, head, row, live), live, g);
   const int32_t* table = p.table + b * p.ld_table;
   w.walk(p, table, 0, (unsigned int) len, W::CHUNK, head, lane);
-  w.close();
   if (live) w.store(0, out_row_of<W::QE>(p, b, head, row), g);
 }
 
@@ -848,7 +847,9 @@ struct SplitArgs {
   int NR;            // row tiles side by side in a workgroup: 1, 2 or 4 waves; the other waves share the positions
   int NG;            // groups of NR * 16 * RT query rows
   int min_run;       // units a workgroup takes at least
-  float* parts;      // [workgroups][2][NR * 16 * RT][D + 4]
+  int blocks;        // workgroups of the split launch
+  float* parts;      // [workgroups][2][NR * 16 * RT][D]
+  float2* part_ml;   // [workgroups][2][NR * 16 * RT]
   int4* meta;        // [workgroups] {sequence (-1: nothing to join), head * NG + group, last workgroup, 0}
 };
 
@@ -907,7 +908,6 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
 
   const int rt = wave % a.NR, ci = wave / a.NR, CI = 4 / a.NR;
   const int group_rows = a.NR * 16 * RT;
-  const int part_ld = D + 4;
   unsigned int b = __builtin_amdgcn_readfirstlane(found[0]);
   unsigned int start = __builtin_amdgcn_readfirstlane(found[1]);
   unsigned int x = x0;
@@ -927,14 +927,13 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
     const int32_t* table = p.table + (int64_t) b * p.ld_table;
     const unsigned int end = ue == u ? (unsigned int) len : ue * UNIT;
     if (row0 < p.rows) w.walk(p, table, ub * UNIT + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
-    w.close();
-    // the waves that shared the positions of a row tile: halves fold together, lane by lane
+      // the waves that shared the positions of a row tile: halves fold together, lane by lane
     for (int half = CI >> 1; half > 0; half >>= 1) {
       const int slot = (ci - half) * a.NR + rt;  // < 2: half * NR <= 2
       if (ci >= half && ci < 2 * half) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          lml[slot][t][lane] = make_float2(w.m[t], w.l[t]);
+          lml[slot][t][lane] = make_float2(w.m[t], w.l[t][0]);
 #pragma unroll
           for (int i = 0; i < W::VH * W::VE; ++i) lo[slot][t * W::VH * W::VE + i][lane] = w.o[t][i / W::VE][i % W::VE];
         }
@@ -947,7 +946,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
           const float2 ml = lml[from][t][lane];
           const Fold k = fold_of(w.m[t], ml.x);
           w.m[t] = k.m;
-          w.l[t] = w.l[t] * k.a + ml.y * k.b;
+          w.l[t][0] = w.l[t][0] * k.a + ml.y * k.b;
 #pragma unroll
           for (int i = 0; i < W::VH * W::VE; ++i)
             w.o[t][i / W::VE][i % W::VE] = w.o[t][i / W::VE][i % W::VE] * k.a + lo[from][t * W::VH * W::VE + i][lane] * k.b;
@@ -957,13 +956,13 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
     }
     if (ci == 0) {
       const bool whole = ub == 0 && ue == u;
-      float* part = a.parts + ((int64_t) blockIdx.x * 2 + (ub == 0 ? 1 : 0)) * group_rows * part_ld;
+      const int64_t part = ((int64_t) blockIdx.x * 2 + (ub == 0 ? 1 : 0)) * group_rows - grp * group_rows;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         const int row = row0 + t * 16 + c;
         if (row < p.rows) {
           if (whole) w.store(t, out_row_of<W::QE>(p, b, head, row), g);
-          else w.store_part(t, part + (int64_t) (row - grp * group_rows) * part_ld, g);
+          else w.store_part(t, a.parts + (part + row) * D, a.part_ml + part + row, g);
         }
       }
       if (threadIdx.x == 0 && ub == 0 && ue < u)
@@ -977,98 +976,87 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   }
 }
 
-// Joins the parts of the (sequence, head, group) that workgroup blockIdx.x began and did not finish: its own second
-// part, then the first parts of the workgroups behind it, in order.  JOIN_WAVES query rows per workgroup, a wave each;
-// of fewer rows several waves take a run of the parts each.
-constexpr int JOIN_WAVES = 4;
+// Joins the parts of the (sequence, head, group) that workgroup `owner` of the split launch began and did not finish: its
+// own second part, then the first parts of the workgroups behind it, in order.  A thread takes four channels of a row and
+// `runs` threads share the parts; eight parts are requested together, and nothing crosses threads but the runs' sums.
+constexpr int JOIN_THREADS = 256;
 
 template <int DT, int D>
-__global__ __launch_bounds__(JOIN_WAVES * 64) void hist_attn_join_kernel(AttnArgs p, SplitArgs a, int group_rows) {
-  constexpr int QE = DT == MI_DT_F32 ? 4 : 2;
-  constexpr int CPL = D >= 64 ? D / 64 : 1;  // channels per lane
-  __shared__ float lacc[JOIN_WAVES][D];
-  __shared__ float2 lml[JOIN_WAVES];
-  const int4 meta = a.meta[blockIdx.x];
-  if (meta.x < 0) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = meta.y / a.NG, grp = meta.y % a.NG;
-  const int n = meta.z - (int) blockIdx.x + 1;
-  const int part_ld = D + 4;
-  const int64_t slot = (int64_t) group_rows * part_ld;
+__global__ __launch_bounds__(JOIN_THREADS) void hist_attn_join_kernel(AttnArgs p, SplitArgs a, int group_rows, int wg_rows) {
+  typedef Wave<DT, D, 1, false> W;
+  constexpr int PIECES = D / 4;
+  __shared__ f4v lacc[JOIN_THREADS];
+  __shared__ float2 lml[JOIN_THREADS];
+  // Workgroups go to the eight XCDs in turn; the ones that have something to join are often every 2nd or 4th of the cut,
+  // so an XCD takes an eighth of the cut as a whole.
+  const int per_xcd = (a.blocks + 7) / 8;
+  const int owner = (int) (blockIdx.x % 8) * per_xcd + (int) (blockIdx.x / 8);
+  if (owner >= a.blocks) return;
+  const int* m4 = reinterpret_cast<const int*>(a.meta + owner);
+  const int b = scalar_load(m4), pair = scalar_load(m4 + 1), n = scalar_load(m4 + 2) - owner + 1;
+  if (b < 0) return;
+  const int head = pair / a.NG, grp = pair % a.NG;
   const int n_rows = p.rows - grp * group_rows < group_rows ? p.rows - grp * group_rows : group_rows;
-  const int r0 = (int) blockIdx.y * JOIN_WAVES;
+  const int r0 = (int) blockIdx.y * wg_rows;
   if (r0 >= n_rows) return;
-  int side = 1;  // rows side by side, a power of two
-  while (side < n_rows - r0 && side < JOIN_WAVES) side <<= 1;
-  const int runs = JOIN_WAVES / side, mine = wave / side;
+  const int t = (int) threadIdx.x, piece = t % PIECES;
+  const int side = PIECES * wg_rows, runs = JOIN_THREADS / side;  // threads of a run; powers of two
+  const int r = r0 + (t & (side - 1)) / PIECES, run = t / side;
+  const bool live = r < n_rows;
+  const int rr = live ? r : r0;
   const int per = (n + runs - 1) / runs;
-  const int i0 = mine * per, i1 = i0 + per < n ? i0 + per : n;
-  const int d = (lane * CPL) & (D - 1);
-  {
-    const int r = r0 + wave % side;
-    const bool live = r < n_rows;
-    float top = -INFINITY, sum = 0.f, acc[CPL];
+  const int i0 = run * per, i1 = i0 + per < n ? i0 + per : n;
+  float top = -INFINITY, sum = 0.f;
+  f4v acc = f4v{0.f, 0.f, 0.f, 0.f};
+  for (int ib = i0; ib < i1; ib += 8) {
+    float2 ml[8];
+    f4v x[8];
 #pragma unroll
-    for (int j = 0; j < CPL; ++j) acc[j] = 0.f;
-    if (live) {
-      const float* first = a.parts + ((int64_t) blockIdx.x * 2 + 1) * slot + (int64_t) r * part_ld;
-      const float* rest = a.parts + (int64_t) blockIdx.x * 2 * slot + (int64_t) r * part_ld;  // part i > 0: + 2 slot i
-      for (int i = i0 + lane; i < i1; i += 64) top = fmaxf(top, (i ? rest + 2 * slot * i : first)[D]);
-      top = mi_wave_max(top);
-      const float base = top == -INFINITY ? 0.f : top;
-      for (int ib = i0; ib < i1; ib += 64) {
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (ib + lane < i1) ml = *reinterpret_cast<const float2*>((ib + lane ? rest + 2 * slot * (ib + lane) : first) + D);
-        const float k = __builtin_amdgcn_exp2f(ml.x - base);
-        sum += ml.y * k;
-        const int m = i1 - ib < 64 ? i1 - ib : 64;
-        // eight parts requested together; behind the last one the last again, unused
-        for (int i = 0; i < m; i += 8) {
-          float x[8][CPL];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int at = ib + (i + e < m ? i + e : m - 1);
-            const float* part = at ? rest + 2 * slot * at : first;
-#pragma unroll
-            for (int j = 0; j < CPL; ++j) x[e][j] = part[d + j];
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float ke = i + e < m ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(k), (i + e) & 63)) : 0.f;
-#pragma unroll
-            for (int j = 0; j < CPL; ++j) acc[j] = i + e < m ? acc[j] + x[e][j] * ke : acc[j];
-          }
-        }
-      }
-      sum = mi_wave_sum(sum);
+    for (int e = 0; e < 8; ++e) {
+      const int i = ib + e < i1 ? ib + e : i1 - 1;  // behind the last part the last again, unused
+      const int64_t at = ((int64_t) (owner + i) * 2 + (i == 0 ? 1 : 0)) * group_rows + rr;
+      ml[e] = a.part_ml[at];
+      x[e] = *reinterpret_cast<const f4v*>(a.parts + at * D + piece * 4);
     }
-    if (runs > 1) {
-      if (lane * CPL < D) {
+    float up = top;
 #pragma unroll
-        for (int j = 0; j < CPL; ++j) lacc[wave][d + j] = acc[j];
+    for (int e = 0; e < 8; ++e)
+      if (ib + e < i1) up = fmaxf(up, ml[e].x);
+    const float base = up == -INFINITY ? 0.f : up;
+    const float k = __builtin_amdgcn_exp2f(top - base);
+    top = up;
+    sum *= k;
+    acc *= k;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (ib + e < i1) {
+        const float w = __builtin_amdgcn_exp2f(ml[e].x - base);
+        sum += ml[e].y * w;
+        acc += x[e] * w;
       }
-      if (lane == 0) lml[wave] = make_float2(top, sum);
-      __syncthreads();
-      if (mine == 0) {
-        for (int k = 1; k < runs; ++k) {
-          const int from = wave + k * side;
-          const float m1 = top, m2 = lml[from].x, m = fmaxf(m1, m2), base = m == -INFINITY ? 0.f : m;
-          const float f1 = __builtin_amdgcn_exp2f(m1 - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
-          top = m;
-          sum = sum * f1 + lml[from].y * f2;
-#pragma unroll
-          for (int j = 0; j < CPL; ++j) acc[j] = acc[j] * f1 + lacc[from][d + j] * f2;
-        }
+  }
+  if (runs > 1) {
+    lacc[t] = acc;
+    lml[t] = make_float2(top, sum);
+    __syncthreads();
+    if (run == 0) {
+      for (int k = 1; k < runs; ++k) {
+        const float2 ml = lml[t + k * side];
+        const Fold f = fold_of(top, ml.x);
+        top = f.m;
+        sum = sum * f.a + ml.y * f.b;
+        acc = acc * f.a + lacc[t + k * side] * f.b;
       }
     }
-    if (live && mine == 0 && lane * CPL < D) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      char* out = out_row_of<QE>(p, meta.x, head, grp * group_rows + r) + d * QE;
+  }
+  if (live && run == 0) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    char* out = out_row_of<W::QE>(p, b, head, grp * group_rows + r);
 #pragma unroll
-      for (int j = 0; j < CPL; ++j) {
-        if (DT == MI_DT_F32) reinterpret_cast<float*>(out)[j] = acc[j] * inv;
-        else reinterpret_cast<unsigned short*>(out)[j] = mi_f2bf(acc[j] * inv);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int d = W::channel_of(piece, e);
+      if (DT == MI_DT_F32) reinterpret_cast<float*>(out)[d] = acc[e] * inv;
+      else reinterpret_cast<unsigned short*>(out)[d] = mi_f2bf(acc[e] * inv);
     }
   }
 }
@@ -1077,7 +1065,7 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void hist_attn_join_kernel(AttnArg
 struct AttnPlan {
   bool short_rows;
   int RT, NR, NG, blocks, min_run;
-  size_t parts_bytes, bytes;
+  size_t parts_bytes, ml_bytes, bytes;
 };
 
 AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int64_t rows, int width) {
@@ -1093,8 +1081,10 @@ AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int
   const int64_t resident = 256 * split_waves(dtype == MI_DT_F32, dim, q.RT);
   q.blocks = (int) (most < resident ? most : resident);
   if (!q.short_rows) {
-    q.parts_bytes = (size_t) q.blocks * 2 * q.NR * 16 * q.RT * (dim + 4) * sizeof(float);
-    q.bytes = q.parts_bytes + (size_t) q.blocks * sizeof(int4);
+    const size_t rows_of_parts = (size_t) q.blocks * 2 * q.NR * 16 * q.RT;
+    q.parts_bytes = rows_of_parts * dim * sizeof(float);
+    q.ml_bytes = rows_of_parts * sizeof(float2);
+    q.bytes = q.parts_bytes + q.ml_bytes + (size_t) q.blocks * sizeof(int4);
   }
   return q;
 }
@@ -1110,14 +1100,18 @@ int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t 
   a.NR = q.NR;
   a.NG = q.NG;
   a.min_run = q.min_run;
+  a.blocks = q.blocks;
   a.parts = (float*) ws;
-  a.meta = (int4*) ((char*) ws + q.parts_bytes);
+  a.part_ml = (float2*) ((char*) ws + q.parts_bytes);
+  a.meta = (int4*) ((char*) ws + q.parts_bytes + q.ml_bytes);
   if (q.RT == 2) hist_attn_split_kernel<DT, D, D <= 128 ? 2 : 1, STREAM><<<q.blocks, 256, 0, s>>>(p, a);
   else hist_attn_split_kernel<DT, D, 1, STREAM><<<q.blocks, 256, 0, s>>>(p, a);
   MI_LAUNCH_CHECK();
-  const int group_rows = q.NR * 16 * q.RT;
-  const dim3 grid(q.blocks, (unsigned int) mi_cdiv(p.rows < group_rows ? p.rows : group_rows, JOIN_WAVES));
-  hist_attn_join_kernel<DT, D><<<grid, JOIN_WAVES * 64, 0, s>>>(p, a, group_rows);
+  const int group_rows = q.NR * 16 * q.RT, side_rows = p.rows < group_rows ? p.rows : group_rows;
+  // few rows can have many parts: four threads share them
+  const int all = JOIN_THREADS / (D / 4), wg_rows = side_rows >= 16 ? all : all / 4;
+  const dim3 grid((q.blocks + 7) / 8 * 8, (unsigned int) mi_cdiv(side_rows, wg_rows));
+  hist_attn_join_kernel<DT, D><<<grid, JOIN_THREADS, 0, s>>>(p, a, group_rows, wg_rows);
   MI_LAUNCH_CHECK();
   return MI_OK;
 }
