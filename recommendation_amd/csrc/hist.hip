@@ -846,10 +846,11 @@ constexpr int UNIT = 128;
 struct SplitArgs {
   int NR;            // row tiles side by side in a workgroup: 1, 2 or 4 waves; the other waves share the positions
   int NG;            // groups of NR * 16 * RT query rows
-  int min_run;       // units a workgroup takes at least
   int blocks;        // workgroups of the split launch
-  float* parts;      // [workgroups][2][NR * 16 * RT][D]
-  float2* part_ml;   // [workgroups][2][NR * 16 * RT]
+  int slot_rows;     // rows of a part: those of a group, or all if there are fewer
+  // Parts: [0] of a workgroup's run continues a row, [1] begins one
+  float* parts;      // [2][workgroups][slot_rows][D]
+  float2* part_ml;   // [2][workgroups][slot_rows]
   int4* meta;        // [workgroups] {sequence (-1: nothing to join), head * NG + group, last workgroup, 0}
 };
 
@@ -889,8 +890,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   }
   before += incl - mine;
   const unsigned int total = all * HG;  // < 2^31, checked on the host
-  unsigned int run = (total + gridDim.x - 1) / gridDim.x;
-  if (run < (unsigned int) a.min_run) run = (unsigned int) a.min_run;
+  const unsigned int run = (total + gridDim.x - 1) / gridDim.x;
   const unsigned int x0 = blockIdx.x * run, x1 = x0 + run < total ? x0 + run : total;
   if (x0 < total && before * HG <= x0 && x0 < (before + mine) * HG) {
     unsigned int b = s0;
@@ -956,7 +956,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
     }
     if (ci == 0) {
       const bool whole = ub == 0 && ue == u;
-      const int64_t part = ((int64_t) blockIdx.x * 2 + (ub == 0 ? 1 : 0)) * group_rows - grp * group_rows;
+      const int64_t part = ((int64_t) (ub == 0 ? gridDim.x : 0) + blockIdx.x) * a.slot_rows - grp * group_rows;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         const int row = row0 + t * 16 + c;
@@ -978,26 +978,19 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
 
 // Joins the parts of the (sequence, head, group) that workgroup `owner` of the split launch began and did not finish: its
 // own second part, then the first parts of the workgroups behind it, in order.  A thread takes four channels of a row and
-// `runs` threads share the parts; eight parts are requested together, and nothing crosses threads but the runs' sums.
+// `runs` threads share the parts; up to eight parts are requested together, and nothing crosses threads but the runs' sums.
 constexpr int JOIN_THREADS = 256;
 
 template <int DT, int D>
-__global__ __launch_bounds__(JOIN_THREADS) void hist_attn_join_kernel(AttnArgs p, SplitArgs a, int group_rows, int wg_rows) {
+__device__ __forceinline__ void join_rows(const AttnArgs& p, const SplitArgs& a, int group_rows, int wg_rows, int slice, int owner,
+                                          f4v* lacc, float2* lml) {
   typedef Wave<DT, D, 1, false> W;
   constexpr int PIECES = D / 4;
-  __shared__ f4v lacc[JOIN_THREADS];
-  __shared__ float2 lml[JOIN_THREADS];
-  // Workgroups go to the eight XCDs in turn; the ones that have something to join are often every 2nd or 4th of the cut,
-  // so an XCD takes an eighth of the cut as a whole.
-  const int per_xcd = (a.blocks + 7) / 8;
-  const int owner = (int) (blockIdx.x % 8) * per_xcd + (int) (blockIdx.x / 8);
-  if (owner >= a.blocks) return;
-  const int* m4 = reinterpret_cast<const int*>(a.meta + owner);
-  const int b = scalar_load(m4), pair = scalar_load(m4 + 1), n = scalar_load(m4 + 2) - owner + 1;
-  if (b < 0) return;
+  const int* meta = reinterpret_cast<const int*>(a.meta + owner);
+  const int b = scalar_load(meta), pair = scalar_load(meta + 1), n = scalar_load(meta + 2) - owner + 1;
   const int head = pair / a.NG, grp = pair % a.NG;
   const int n_rows = p.rows - grp * group_rows < group_rows ? p.rows - grp * group_rows : group_rows;
-  const int r0 = (int) blockIdx.y * wg_rows;
+  const int r0 = slice * wg_rows;
   if (r0 >= n_rows) return;
   const int t = (int) threadIdx.x, piece = t % PIECES;
   const int side = PIECES * wg_rows, runs = JOIN_THREADS / side;  // threads of a run; powers of two
@@ -1006,22 +999,27 @@ __global__ __launch_bounds__(JOIN_THREADS) void hist_attn_join_kernel(AttnArgs p
   const int rr = live ? r : r0;
   const int per = (n + runs - 1) / runs;
   const int i0 = run * per, i1 = i0 + per < n ? i0 + per : n;
+  const float* sums = a.parts + rr * D + piece * 4;
+  const float2* mls = a.part_ml + rr;
   float top = -INFINITY, sum = 0.f;
   f4v acc = f4v{0.f, 0.f, 0.f, 0.f};
   for (int ib = i0; ib < i1; ib += 8) {
     float2 ml[8];
     f4v x[8];
+    const int m = i1 - ib;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int i = ib + e < i1 ? ib + e : i1 - 1;  // behind the last part the last again, unused
-      const int64_t at = ((int64_t) (owner + i) * 2 + (i == 0 ? 1 : 0)) * group_rows + rr;
-      ml[e] = a.part_ml[at];
-      x[e] = *reinterpret_cast<const f4v*>(a.parts + at * D + piece * 4);
+      ml[e] = make_float2(-INFINITY, 0.f);
+      x[e] = f4v{0.f, 0.f, 0.f, 0.f};
+      if (e < m) {
+        const unsigned int at = (unsigned int) (owner + ib + e + (ib + e == 0 ? a.blocks : 0)) * (unsigned int) a.slot_rows;
+        ml[e] = mls[at];
+        x[e] = *reinterpret_cast<const f4v*>(sums + (uint64_t) at * D);
+      }
     }
     float up = top;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (ib + e < i1) up = fmaxf(up, ml[e].x);
+    for (int e = 0; e < 8; ++e) up = fmaxf(up, ml[e].x);
     const float base = up == -INFINITY ? 0.f : up;
     const float k = __builtin_amdgcn_exp2f(top - base);
     top = up;
@@ -1029,13 +1027,14 @@ __global__ __launch_bounds__(JOIN_THREADS) void hist_attn_join_kernel(AttnArgs p
     acc *= k;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (ib + e < i1) {
+      if (e < m) {
         const float w = __builtin_amdgcn_exp2f(ml[e].x - base);
         sum += ml[e].y * w;
         acc += x[e] * w;
       }
   }
   if (runs > 1) {
+    __syncthreads();  // the rows before have been read
     lacc[t] = acc;
     lml[t] = make_float2(top, sum);
     __syncthreads();
@@ -1061,10 +1060,29 @@ __global__ __launch_bounds__(JOIN_THREADS) void hist_attn_join_kernel(AttnArgs p
   }
 }
 
+template <int DT, int D>
+__global__ __launch_bounds__(JOIN_THREADS) void hist_attn_join_kernel(AttnArgs p, SplitArgs a, int group_rows, int wg_rows,
+                                                                     int slices) {
+  __shared__ f4v lacc[JOIN_THREADS];
+  __shared__ float2 lml[JOIN_THREADS];
+  // Workgroups go to the 256 CUs in turn (the eight XCDs, and there their CUs), and the owners with something to join are
+  // often every 2nd, 4th or 8th: a CU takes a stretch of owners as a whole, another one with each slice of their rows, so
+  // they do not meet on a few (64 rows x 2 parts x 128 heads: 22 us in the order of the owners, 8 so).  `subs` workgroups
+  // share the stretch: a workgroup costs the launch about 1 ns, whether it finds something to do or not.
+  const int per_cu = (a.blocks + 255) / 256, subs = (int) gridDim.x / 256 / slices;
+  const int slice = (int) blockIdx.x / (256 * subs), sub = (int) blockIdx.x / 256 % subs;
+  const int first = ((int) blockIdx.x + slice * 37) % 256 * per_cu + sub;
+  const int lane = (int) threadIdx.x & 63, mine = first + lane * subs;
+  uint64_t todo = __ballot(sub + lane * subs < per_cu && mine < a.blocks && a.meta[mine < a.blocks ? mine : 0].x >= 0);
+  for (; todo; todo &= todo - 1)
+    join_rows<DT, D>(p, a, group_rows, wg_rows, slice,
+                     __builtin_amdgcn_readfirstlane(first + (__ffsll((unsigned long long) todo) - 1) * subs), lacc, lml);
+}
+
 // How a call is run; the same on every call of the same sizes.
 struct AttnPlan {
   bool short_rows;
-  int RT, NR, NG, blocks, min_run;
+  int RT, NR, NG, blocks, slot_rows;
   size_t parts_bytes, ml_bytes, bytes;
 };
 
@@ -1076,14 +1094,15 @@ AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int
   q.NR = tiles >= 3 ? 4 : (int) tiles;
   q.NG = (int) mi_cdiv(tiles, q.NR);
   q.short_rows = room <= 256;
-  q.min_run = 1;
   const int64_t most = n_seqs * H * q.NG * mi_cdiv(room, UNIT);
   const int64_t resident = 256 * split_waves(dtype == MI_DT_F32, dim, q.RT);
   q.blocks = (int) (most < resident ? most : resident);
   if (!q.short_rows) {
-    const size_t rows_of_parts = (size_t) q.blocks * 2 * q.NR * 16 * q.RT;
-    q.parts_bytes = rows_of_parts * dim * sizeof(float);
-    q.ml_bytes = rows_of_parts * sizeof(float2);
+    const int64_t group_rows = q.NR * 16 * q.RT;
+    q.slot_rows = (int) (rows < group_rows ? rows : group_rows);
+    const size_t part_rows = (size_t) q.blocks * 2 * q.slot_rows;
+    q.parts_bytes = part_rows * dim * sizeof(float);
+    q.ml_bytes = (part_rows * sizeof(float2) + 15) / 16 * 16;
     q.bytes = q.parts_bytes + q.ml_bytes + (size_t) q.blocks * sizeof(int4);
   }
   return q;
@@ -1099,19 +1118,19 @@ int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t 
   SplitArgs a = {};
   a.NR = q.NR;
   a.NG = q.NG;
-  a.min_run = q.min_run;
   a.blocks = q.blocks;
+  a.slot_rows = q.slot_rows;
   a.parts = (float*) ws;
   a.part_ml = (float2*) ((char*) ws + q.parts_bytes);
   a.meta = (int4*) ((char*) ws + q.parts_bytes + q.ml_bytes);
   if (q.RT == 2) hist_attn_split_kernel<DT, D, D <= 128 ? 2 : 1, STREAM><<<q.blocks, 256, 0, s>>>(p, a);
   else hist_attn_split_kernel<DT, D, 1, STREAM><<<q.blocks, 256, 0, s>>>(p, a);
   MI_LAUNCH_CHECK();
-  const int group_rows = q.NR * 16 * q.RT, side_rows = p.rows < group_rows ? p.rows : group_rows;
-  // few rows can have many parts: four threads share them
-  const int all = JOIN_THREADS / (D / 4), wg_rows = side_rows >= 16 ? all : all / 4;
-  const dim3 grid((q.blocks + 7) / 8 * 8, (unsigned int) mi_cdiv(side_rows, wg_rows));
-  hist_attn_join_kernel<DT, D><<<grid, JOIN_THREADS, 0, s>>>(p, a, group_rows, wg_rows);
+  // few rows can have many parts: several threads share them
+  const int all = JOIN_THREADS / (D / 4), wg_rows = q.slot_rows >= 16 ? all : (all / 4 + 1) / 2;
+  const int slices = (int) mi_cdiv(q.slot_rows, wg_rows), per_cu = (int) mi_cdiv(q.blocks, 256);
+  const int subs = slices >= 8 ? 1 : 8 / slices < per_cu ? 8 / slices : per_cu;
+  hist_attn_join_kernel<DT, D><<<256 * subs * slices, JOIN_THREADS, 0, s>>>(p, a, q.NR * 16 * q.RT, wg_rows, slices);
   MI_LAUNCH_CHECK();
   return MI_OK;
 }
