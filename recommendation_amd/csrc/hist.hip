@@ -366,6 +366,7 @@ int launch_rows(const RowArgs& p, int dim, hipStream_t s) {
   int shift = 0;
   while ((2 * p.H) << shift < groups && shift < 6) ++shift;
   while (shift < 2 && (p.n_rows >> (shift + 1)) >= 4096) ++shift;
+  while (shift < 6 && (p.n_rows >> shift) > (1 << 25)) ++shift;  // a launch holds less than 2^32 threads
   const dim3 grid((unsigned int) mi_cdiv(p.n_rows, 4ll << shift));
   const bool stream = p.n_rows * 2 * p.H * dim * (Elem<CT>::BYTES + Elem<IT>::BYTES) > LAST_LEVEL_BYTES;
 #define MI_HIST_ROWS(D)                                                                            \
@@ -392,7 +393,7 @@ struct AttnArgs {
   int64_t q_seq, q_tok, q_head;  // strides in elements
   char* out;
   int64_t o_seq, o_tok, o_head;
-  int G, rows, n_rt;             // query heads per cache head; n_q * G query rows per cache head, in tiles of 16
+  int G, rows;                   // query heads per cache head; n_q * G query rows per cache head
   const int32_t* table;
   int64_t ld_table;
   int width;
@@ -557,28 +558,27 @@ struct Wave {
 
   // All chunks pos, pos + stride, ... < end.  A chunk's page ids are requested two steps ahead, its K while the values
   // of the chunk before are summed, its V while its own scores are formed: one set of registers, and loads in flight all
-  // the time.  Behind the end the last chunk is requested again (from the caches): a load that some steps skip would
-  // make every step wait for all loads.
+  // the time.  The last chunk stands behind the loop: loads that only some steps issue would make every step wait for all.
   __device__ __forceinline__ void walk(const AttnArgs& p, const int32_t* table, unsigned int pos, unsigned int end,
                                        unsigned int stride, int head, int lane) {
     if (pos >= end) return;
     Fetched f;
+    f4v s[RT][2];
     Where at = locate(p, look(p, table, pos, end), head, lane);
-    Ahead ahead = look(p, table, pos + stride, end);
     request_k(f, p, at, lane);
     request_v(f, p, at, lane);
-    for (;;) {
+    Ahead ahead = look(p, table, pos + stride, end);
+    for (; pos + stride < end; pos += stride) {
       const Where next = locate(p, ahead, head, lane);
       ahead = look(p, table, pos + 2 * stride, end);
-      f4v s[RT][2];
       scores(s, f, p);
       request_k(f, p, next, lane);
       weigh(s, f, at, lane);
       request_v(f, p, next, lane);
-      pos += stride;
-      if (pos >= end) break;
       at = next;
     }
+    scores(s, f, p);
+    weigh(s, f, at, lane);
   }
 
   static __device__ __forceinline__ bf8v widen(unsigned int lo, unsigned int hi) {  // 8 e4m3 codes, exactly
@@ -816,25 +816,31 @@ __device__ __forceinline__ int64_t clamped_length(const AttnArgs& p, int32_t len
   return len > room ? room : (len < 0 ? 0 : len);
 }
 
-// Short histories: one wave per (sequence, cache head, tile of 16 query rows).
-template <int DT, int D, bool STREAM>
-__global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, 1)) void hist_attn_short_kernel(AttnArgs p) {
-  typedef Wave<DT, D, 1, STREAM> W;
+// Short histories: one wave per (sequence, cache head, RT tiles of 16 query rows).  Through the caches whatever the pool's
+// size: the waves of further row tiles come right behind (35 rows over 27 positions: 149 us so, 187 past them).
+template <int DT, int D, int RT>
+__global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist_attn_short_kernel(AttnArgs p, int n_tiles) {
+  typedef Wave<DT, D, RT, false> W;
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const unsigned int seg = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned int pair = seg / (unsigned int) p.n_rt;
-  const int rt = (int) (seg - pair * p.n_rt);
+  const unsigned int pair = seg / (unsigned int) n_tiles;
+  const int row0 = (int) (seg - pair * n_tiles) * 16 * RT;
   const int64_t b = pair / (unsigned int) p.H;
   const int head = (int) (pair - (unsigned int) b * p.H);
   if (b >= p.n_seqs) return;
   const int64_t len = clamped_length(p, scalar_load(p.lengths + b), lane == 0);
-  const int row = rt * 16 + c;
-  const bool live = row < p.rows;
   W w;
-  w.init(0, q_row_of<W::QE>(p, b, head, row, live), live, g);
-  const int32_t* table = p.table + b * p.ld_table;
-  w.walk(p, table, 0, (unsigned int) len, W::CHUNK, head, lane);
-  if (live) w.store(0, out_row_of<W::QE>(p, b, head, row), g);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int row = row0 + t * 16 + c;
+    w.init(t, q_row_of<W::QE>(p, b, head, row, row < p.rows), row < p.rows, g);
+  }
+  w.walk(p, p.table + b * p.ld_table, 0, (unsigned int) len, W::CHUNK, head, lane);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int row = row0 + t * 16 + c;
+    if (row < p.rows) w.store(t, out_row_of<W::QE>(p, b, head, row), g);
+  }
 }
 
 // Long histories: the call's work is cut into equal runs of units, a unit being UNIT positions of one (sequence, cache
@@ -1108,13 +1114,18 @@ AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int
   return q;
 }
 
+template <int DT, int D>
+int launch_short(const AttnArgs& p, const AttnPlan& q, hipStream_t s) {
+  const int n_tiles = (int) mi_cdiv(p.rows, 16 * q.RT);
+  const dim3 grid((unsigned int) mi_cdiv(p.n_seqs * p.H * n_tiles, 4));
+  if (q.RT == 2) hist_attn_short_kernel<DT, D, D <= 128 ? 2 : 1><<<grid, 256, 0, s>>>(p, n_tiles);
+  else hist_attn_short_kernel<DT, D, 1><<<grid, 256, 0, s>>>(p, n_tiles);
+  MI_LAUNCH_CHECK();
+  return MI_OK;
+}
+
 template <int DT, int D, bool STREAM>
-int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) {
-  if (q.short_rows) {
-    hist_attn_short_kernel<DT, D, STREAM><<<dim3((unsigned int) mi_cdiv(p.n_seqs * p.H * p.n_rt, 4)), 256, 0, s>>>(p);
-    MI_LAUNCH_CHECK();
-    return MI_OK;
-  }
+int launch_split(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) {
   SplitArgs a = {};
   a.NR = q.NR;
   a.NG = q.NG;
@@ -1135,14 +1146,24 @@ int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t 
   return MI_OK;
 }
 
+template <int DT, int D>
+int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) {
+  if (q.short_rows) return launch_short<DT, D>(p, q, s);
+  // past the caches where the pool does not fit the last one (64 bf16 histories of 8-16 k: 479 us so, 537 through them;
+  // the other way round 72 MB of candidates' histories: 57 against 48) and no second row tile reads the same positions
+  // (16 candidates each for 256 users: 199 us past the caches, 165 through them)
+  const bool stream = ((int64_t) p.n_pages * p.H * 2 << p.page_shift) * D * Elem<DT>::BYTES > LAST_LEVEL_BYTES &&
+                      q.NR == 1 && q.NG == 1;
+  return stream ? launch_split<DT, D, true>(p, q, ws, s) : launch_split<DT, D, false>(p, q, ws, s);
+}
+
 template <int DT>
 int launch_attn(const AttnArgs& p, const AttnPlan& q, int dim, void* ws, hipStream_t s) {
-  const bool stream = ((int64_t) p.n_pages * p.H * 2 << p.page_shift) * dim * Elem<DT>::BYTES > LAST_LEVEL_BYTES;
   switch (dim) {
-    case 32: return stream ? launch_attn_dim<DT, 32, true>(p, q, ws, s) : launch_attn_dim<DT, 32, false>(p, q, ws, s);
-    case 64: return stream ? launch_attn_dim<DT, 64, true>(p, q, ws, s) : launch_attn_dim<DT, 64, false>(p, q, ws, s);
-    case 128: return stream ? launch_attn_dim<DT, 128, true>(p, q, ws, s) : launch_attn_dim<DT, 128, false>(p, q, ws, s);
-    default: return stream ? launch_attn_dim<DT, 256, true>(p, q, ws, s) : launch_attn_dim<DT, 256, false>(p, q, ws, s);
+    case 32: return launch_attn_dim<DT, 32>(p, q, ws, s);
+    case 64: return launch_attn_dim<DT, 64>(p, q, ws, s);
+    case 128: return launch_attn_dim<DT, 128>(p, q, ws, s);
+    default: return launch_attn_dim<DT, 256>(p, q, ws, s);
   }
 }
 
@@ -1296,7 +1317,6 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
   const int64_t rows = (int64_t) n_queries * p.G;
   MI_REQUIRE(rows <= 65536, "mi_hist_attn: %lld query rows per cache head (at most 65536)", (long long) rows);
   p.rows = (int) rows;
-  p.n_rt = (int) mi_cdiv(rows, 16);
   p.table = page_table;
   p.ld_table = ld_table;
   p.width = table_width;
@@ -1305,10 +1325,12 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
   p.scale = scale * 1.44269504088896340736f;
   p.err = err;
   const AttnPlan plan = plan_attn(cache->dtype, cache->dim, p.H, cache->page_size, n_seqs, rows, table_width);
-  // unit and segment numbers are 32-bit in the kernels
-  if (mi_cdiv((int64_t) table_width * cache->page_size, UNIT) > INT32_MAX / (n_seqs * p.H) / p.n_rt) {
-    mi_set_error("mi_hist_attn: %lld sequences x %d heads x %d row tiles over %d pages in one call", (long long) n_seqs, p.H,
-                 p.n_rt, table_width);
+  // unit numbers are 32-bit in the kernels
+  const int64_t tiles = mi_cdiv(rows, 16);
+  if (n_seqs * p.H > (1 << 25) / tiles ||  // waves of a launch
+      mi_cdiv((int64_t) table_width * cache->page_size, UNIT) > INT32_MAX / (n_seqs * p.H * tiles)) {
+    mi_set_error("mi_hist_attn: %lld sequences x %d heads x %lld row tiles over %d pages in one call", (long long) n_seqs, p.H,
+                 (long long) tiles, table_width);
     return MI_ERR_UNSUPPORTED;
   }
   if (plan.bytes) {

@@ -1117,7 +1117,7 @@ def hist_read(cache, page_table, lengths, n_rows=None, offsets=None, dtype=torch
 def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
     """Softmax attention of every sequence's new tokens or candidates ``q`` [sequences, heads, dim] or [sequences, tokens,
     heads, dim] over all ``lengths`` positions of its history; the query heads share the cache's heads in equal groups.
-    q: float32 over a float32 cache, bfloat16 otherwise; the result has its shape and type.  ``scale``: of the scores,
+    q: float32 over a float32 cache, bfloat16 otherwise; the result has its shape and type (``out`` may be q itself).  ``scale``: of the scores,
     dim ** -0.5 by default.  A sequence without history gives zeros."""
     n, width, ld_table = _hist_common('hist_attn', cache, page_table, lengths, None, err, q, out)
     shape, dtype, heads, dim = q.shape, q.dtype, cache.n_heads, cache.dim

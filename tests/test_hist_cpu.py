@@ -127,6 +127,33 @@ def test_bad_attention_calls_are_refused():
     assert rc(tokens=0)[0] == 0 and rc(seqs=0)[0] == 0
 
 
+def test_attention_workspace_is_checked():
+    """Histories of up to 256 positions need none; beyond, what mi_hist_attn_workspace_bytes says."""
+    from recommendation_amd import _lib
+    lib = _lib.load()
+    c = _cache()
+    need = lambda **kw: lib.mi_hist_attn_workspace_bytes(ctypes.byref(_cache(**kw.pop('cache', {}))), kw.pop('seqs', 4), kw.pop('tokens', 1),
+                                                         kw.pop('heads', 2), kw.pop('width', 17))
+    assert need(width=16) == 0 and need() > 0
+    assert need(seqs=0) == need(tokens=0) == need(heads=3) == need(width=0) == need(cache=dict(dim=48)) == 0
+    assert need(seqs=4096, width=4096) < 1 << 26
+
+    def rc(ws, ws_bytes, width=17, seqs=4, ld=100000000, tokens=1):
+        code = lib.mi_hist_attn(ctypes.byref(c), 4096, 128, 128, 64, 2, tokens, seqs, 4096, ld, width, 4096, 0.1, 4096, 128, 128,
+                                64, ws, ws_bytes, None, None)
+        return code, lib.mi_last_error().decode()
+
+    for ws, n in ((None, 0), (None, 1 << 30), (4096, need() - 1), (4096, 0)):
+        code, msg = rc(ws, n)
+        assert code == -3 and 'workspace' in msg and str(need()) in msg, (ws, n, msg)
+    code, msg = rc(4104, 1 << 30)
+    assert code == -1 and 'aligned' in msg
+    # more work than one launch can number
+    for kw in (dict(seqs=1 << 26), dict(width=100000000, seqs=1 << 10), dict(seqs=1 << 14, tokens=65536)):
+        code, msg = rc(4096, 1 << 40, **kw)
+        assert code == -4 and 'in one call' in msg, (kw, code, msg)
+
+
 def test_host_tensors_are_refused():
     from recommendation_amd import ops
     with pytest.raises(ops.MiError, match='device tensors'):

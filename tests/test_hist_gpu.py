@@ -246,7 +246,8 @@ def test_attention_at_every_edge_of_tile_and_page(dev, cache, dim):
 @pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
 @pytest.mark.parametrize('lens, heads, group, tokens, dim, page', [
     ([5000], 1, 1, 1, 64, 16), ([1023, 1, 0, 4097], 2, 8, 1, 128, 64), ([3000, 10, 2999], 1, 16, 1, 64, 1024),
-    ([2500, 700], 2, 3, 11, 32, 32), ([1500, 1], 1, 1, 70, 256, 16), ([900] * 40, 4, 2, 1, 64, 16)])
+    ([2500, 700], 2, 3, 11, 32, 32), ([1500, 1], 1, 1, 70, 256, 16), ([900] * 40, 4, 2, 1, 64, 16),
+    ([700, 31, 400], 1, 1, 150, 64, 16), ([300, 290], 2, 1, 40, 128, 32), ([40000, 5], 1, 2, 1, 32, 256)])
 def test_attention_over_long_histories(dev, cache, lens, heads, group, tokens, dim, page):
     run_attn(dev, np.random.default_rng(len(lens) + dim), cache, lens, page, heads, group, tokens, dim)
 
@@ -257,6 +258,69 @@ def test_attention_of_many_short_histories(dev, cache):
     rng = np.random.default_rng(9)
     lens = rng.integers(0, 101, size=1500).tolist()
     run_attn(dev, rng, cache, lens, 16, 1, 1, 1, 64, width=7)
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_attention_of_many_uneven_histories(dev, cache):
+    """More sequences than a workgroup has threads, lengths below zero, runs of empty ones, histories that end anywhere
+    in a run of the cut."""
+    rng = np.random.default_rng(10)
+    lens = rng.integers(0, 600, size=700)
+    lens[100:160] = 0
+    lens[200:400] = rng.integers(-3, 3, size=200)
+    lens[-1], lens[0] = 3001, 1
+    run_attn(dev, rng, cache, lens.tolist(), 16, 1, 2, 1, 32)
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('dim', [32, 64, 128, 256])
+def test_pools_beyond_the_last_level_cache(dev, cache, dim):
+    """A pool of more than 256 MB is read past the caches; same sums, bit for bit, as over the same pages in a small one."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(dim + 1)
+    page, heads, lens = 64, 2, [700, 0, 1, 1500]
+    c, table, lengths, t = filled(dev, rng, cache, lens, page, heads, dim)
+    per_page = heads * 2 * page * dim * c.kv.element_size()
+    n_pages = (300 << 20) // per_page + c.n_pages
+    big = poisoned(dev, cache, n_pages, page, heads, dim)
+    lo = n_pages - c.n_pages
+    big.kv.view(torch.uint8)[lo:] = c.kv.view(torch.uint8)
+    if cache == 'e4m3':
+        big.exps[lo:] = c.exps
+    moved = torch.where(table >= 0, table + lo, table)
+    dt = torch.float32 if cache == 'f32' else torch.bfloat16
+    for shape in ((4, 6, dim), (4, 9, 4, dim)):
+        q = torch.from_numpy(rng.standard_normal(shape)).to(dev, dt)
+        assert torch.equal(ops.hist_attn(big, q, moved, lengths), ops.hist_attn(c, q, table, lengths))
+
+
+@pytest.mark.parametrize('cache, given', [('f32', torch.float32), ('bf16', torch.bfloat16), ('e4m3', torch.float32),
+                                          ('e4m3', torch.bfloat16)])
+def test_rows_beyond_the_last_level_cache(dev, cache, given):
+    """A call that moves more than 256 MB goes past the caches; same bits as two calls of half the rows."""
+    from recommendation_amd import ops
+    gen = torch.Generator(device=dev).manual_seed(3)
+    heads, dim, page, users, each = 8, 256, 256, 8, 5001
+    width = -(-each // page)
+    rows = torch.randn((users * each, 2, heads, dim), generator=gen, device=dev).to(given)
+    assert rows.numel() * (rows.element_size() + DTYPES[cache].itemsize) > 256 << 20
+    table = torch.randperm(users * width, generator=gen, device=dev).to(torch.int32).view(users, width)
+    lengths = torch.full((users,), each, dtype=torch.int32, device=dev)
+    whole, halves = (poisoned(dev, cache, users * width, page, heads, dim) for _ in range(2))
+    ops.hist_write(whole, rows[:, 0], rows[:, 1], table, lengths)
+    h = users // 8
+    for b in range(0, users, h):
+        part = rows[b * each:(b + h) * each]
+        ops.hist_write(halves, part[:, 0], part[:, 1], table[b:b + h], lengths[b:b + h])
+    assert torch.equal(whole.kv.view(torch.uint8), halves.kv.view(torch.uint8))
+    if cache == 'e4m3':
+        assert torch.equal(whole.exps, halves.exps)
+    k, v = ops.hist_read(whole, table, lengths, users * each, dtype=given)
+    for b in range(0, users, h):
+        k1, v1 = ops.hist_read(whole, table[b:b + h], lengths[b:b + h], h * each, dtype=given)
+        assert torch.equal(k[b * each:(b + h) * each], k1) and torch.equal(v[b * each:(b + h) * each], v1)
+    if cache != 'e4m3':
+        assert torch.equal(k, rows[:, 0]) and torch.equal(v, rows[:, 1])
 
 
 @pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
@@ -405,6 +469,49 @@ def test_histories_grow_event_by_event(dev, cache):
     fresh = poisoned(dev, cache, users * width, page, heads, dim)
     ops.hist_write(fresh, k2, v2, table, final, offsets=offs)
     np.testing.assert_array_equal(values(fresh), values(c))
+
+
+def test_captured_attention_over_long_histories(dev):
+    """The two launches and the workspace between them inside graphs: two graphs captured one after the other, replayed in
+    turn on two streams with new lengths and queries, eager calls between; every replay equals the eager call."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(14)
+    c, table, lengths, t = filled(dev, rng, 'bf16', [3000, 2900, 1, 600, 0], 16, 2, 128)
+    full = lengths.clone()
+    qs = [torch.from_numpy(rng.standard_normal((5, 8, 128))).to(dev, torch.bfloat16) for _ in range(2)]
+    outs = [torch.zeros_like(q) for q in qs]
+    lens = [full.clone(), full.clone()]
+    ops.hist_attn(c, qs[0], table, full)
+    torch.cuda.synchronize()
+    graphs = []
+    for q, out, n in zip(qs, outs, lens):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.hist_attn(c, q, table, n, out=out)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for step in range(6):
+        for i in range(2):
+            qs[i].copy_(torch.from_numpy(rng.standard_normal((5, 8, 128))))
+            lens[i].copy_(torch.clamp(full - int(rng.integers(0, 500)), min=0))
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        eager = [ops.hist_attn(c, qs[i], table, lens[i]) for i in range(2)]
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], eager[0]) and torch.equal(outs[1], eager[1])
+        assert not eager[0][4].any()
+
+
+def test_the_result_may_replace_the_queries(dev):
+    from recommendation_amd import ops
+    rng = np.random.default_rng(15)
+    for lens in ([50, 3, 0], [4000, 70, 900]):
+        c, table, lengths, t = filled(dev, rng, 'e4m3', lens, 16, 2, 64)
+        q = torch.from_numpy(rng.standard_normal((3, 20, 6, 64))).to(dev, torch.bfloat16)
+        want = ops.hist_attn(c, q, table, lengths)
+        assert ops.hist_attn(c, q, table, lengths, out=q) is q and torch.equal(q, want)
 
 
 def test_two_calls_at_once_on_two_streams(dev):
