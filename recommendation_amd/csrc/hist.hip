@@ -847,7 +847,12 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
 // head, group of query rows), sequences slowest; a workgroup walks its run.  A run that begins or ends inside a
 // (sequence, head, group) leaves an unnormalised part, which the joining launch adds up.  The cut goes by the lengths
 // alone, so histories of any mix keep every workgroup equally busy, and the parts are always joined in the same order.
-constexpr int UNIT = 128;
+constexpr unsigned int UNIT = 128;
+// Runs of up to ALIGN_RUN units begin and end with a row of work instead, where the chip can hold them all: a second row
+// in a workgroup costs it a second start (lengths, pages, queries, the first positions: some 6 us), more than the uneven
+// pieces do.  A unit is then that many times longer, and a run one unit.  (16 candidates each for 32 users: 38 us with
+// runs that cross rows, 35 so.)
+constexpr unsigned int ALIGN_RUN = 8;
 
 struct SplitArgs {
   int NR;            // row tiles side by side in a workgroup: 1, 2 or 4 waves; the other waves share the positions
@@ -860,8 +865,8 @@ struct SplitArgs {
   int4* meta;        // [workgroups] {sequence (-1: nothing to join), head * NG + group, last workgroup, 0}
 };
 
-__device__ __forceinline__ unsigned int units_of(int64_t len) {
-  return len <= UNIT ? 1u : (unsigned int) ((len + UNIT - 1) / UNIT);
+__device__ __forceinline__ unsigned int units_of(int64_t len, unsigned int unit) {
+  return len <= unit ? 1u : ((unsigned int) len + unit - 1) / unit;
 }
 
 template <int DT, int D, int RT, bool STREAM>
@@ -875,33 +880,46 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned int HG = (unsigned int) (p.H * a.NG), n_seqs = (unsigned int) p.n_seqs;
 
-  // units in front of each thread's slice of the sequences
+  // units in front of each thread's slice of the sequences, and all
   const unsigned int per = (n_seqs + 255) / 256;
   const unsigned int s0 = threadIdx.x * per, s1 = s0 + per < n_seqs ? s0 + per : n_seqs;
-  unsigned int mine = 0;
-  for (unsigned int b = s0; b < s1; ++b) mine += units_of(clamped_length(p, p.lengths[b], blockIdx.x == 0));
-  unsigned int incl = mine;
+  unsigned int unit = UNIT, before, mine, total;
+  auto count = [&](bool say) {
+    mine = 0;
+    for (unsigned int b = s0; b < s1; ++b) mine += units_of(clamped_length(p, p.lengths[b], say), unit);
+    unsigned int incl = mine;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned int up = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 63) wave_sum[wave] = incl;
-  __syncthreads();
-  unsigned int before = 0, all = 0;
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned int up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 63) wave_sum[wave] = incl;
+    __syncthreads();
+    before = 0;
+    total = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < wave) before += wave_sum[i];
-    all += wave_sum[i];
+    for (int i = 0; i < 4; ++i) {
+      if (i < wave) before += wave_sum[i];
+      total += wave_sum[i];
+    }
+    before += incl - mine;
+    total = __builtin_amdgcn_readfirstlane(total) * HG;  // < 2^31, checked on the host
+  };
+  count(blockIdx.x == 0);
+  unsigned int run = (total + gridDim.x - 1) / gridDim.x;
+  if (run > 1 && run <= ALIGN_RUN && 2 * HG * n_seqs <= gridDim.x) {
+    for (unsigned int k = run; total > gridDim.x; ++k) {  // at 2 * run at the latest they fit
+      __syncthreads();  // wave_sum has been read
+      unit = UNIT * k;
+      count(false);
+    }
+    run = 1;
   }
-  before += incl - mine;
-  const unsigned int total = all * HG;  // < 2^31, checked on the host
-  const unsigned int run = (total + gridDim.x - 1) / gridDim.x;
   const unsigned int x0 = blockIdx.x * run, x1 = x0 + run < total ? x0 + run : total;
   if (x0 < total && before * HG <= x0 && x0 < (before + mine) * HG) {
     unsigned int b = s0;
     for (;; ++b) {
-      const unsigned int u = units_of(clamped_length(p, p.lengths[b], false));
+      const unsigned int u = units_of(clamped_length(p, p.lengths[b], false), unit);
       if (x0 < (before + u) * HG) break;
       before += u;
     }
@@ -919,7 +937,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   unsigned int x = x0;
   while (x < x1) {
     const int64_t len = clamped_length(p, scalar_load(p.lengths + b), false);
-    const unsigned int u = units_of(len);
+    const unsigned int u = units_of(len, unit);
     const unsigned int rem = x - start, pair = rem / u, ub = rem - pair * u;
     const int head = (int) (pair / (unsigned int) a.NG), grp = (int) (pair - (unsigned int) head * a.NG);
     const unsigned int ue = ub + (x1 - x) < u ? ub + (x1 - x) : u;
@@ -931,8 +949,8 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
       w.init(t, q_row_of<W::QE>(p, b, head, row, row < p.rows), row < p.rows, g);
     }
     const int32_t* table = p.table + (int64_t) b * p.ld_table;
-    const unsigned int end = ue == u ? (unsigned int) len : ue * UNIT;
-    if (row0 < p.rows) w.walk(p, table, ub * UNIT + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
+    const unsigned int end = ue == u ? (unsigned int) len : ue * unit;
+    if (row0 < p.rows) w.walk(p, table, ub * unit + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
       // the waves that shared the positions of a row tile: halves fold together, lane by lane
     for (int half = CI >> 1; half > 0; half >>= 1) {
       const int slot = (ci - half) * a.NR + rt;  // < 2: half * NR <= 2
