@@ -361,11 +361,13 @@ __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shi
 
 template <int CT, int IT, bool READ>
 int launch_rows(const RowArgs& p, int dim, hipStream_t s) {
-  // at least the rows of one instruction; beyond that, more tokens a wave as long as there are four waves for every SIMD
+  // at least the rows of one instruction; beyond that up to four tokens a wave as long as there are four waves for every
+  // SIMD.  f32 rows leave a wave token by token: 8 KB at a time then (65 k rows of 8 x 128 read back: 103 us, 119 with
+  // four tokens a wave; in bf16 287 and 280, written from bf16 102 and 88).
   const int groups = 64 / (dim / 8);
   int shift = 0;
   while ((2 * p.H) << shift < groups && shift < 6) ++shift;
-  while (shift < 2 && (p.n_rows >> (shift + 1)) >= 4096) ++shift;
+  while (shift < (READ && IT == MI_DT_F32 ? 0 : 2) && (p.n_rows >> (shift + 1)) >= 4096) ++shift;
   while (shift < 6 && (p.n_rows >> shift) > (1 << 25)) ++shift;  // a launch holds less than 2^32 threads
   const dim3 grid((unsigned int) mi_cdiv(p.n_rows, 4ll << shift));
   const bool stream = p.n_rows * 2 * p.H * dim * (Elem<CT>::BYTES + Elem<IT>::BYTES) > LAST_LEVEL_BYTES;
