@@ -536,8 +536,10 @@ struct Wave {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const char* kb = p.kv + w.rows[t] * (D * E);
+      const unsigned int most = w.valid[t] > 0 ? w.valid[t] - 1 : 0;  // behind the end the last row again
+      const unsigned int row = c < most ? c : most;
 #pragma unroll
-      for (int s = 0; s < KL; ++s) fetch<KB>(f.k[t][s], kb + s * (KB * 4) + (c * (D * E) + g * KB));
+      for (int s = 0; s < KL; ++s) fetch<KB>(f.k[t][s], kb + s * (KB * 4) + (row * (D * E) + g * KB));
       if (DT == MI_DT_E4M3) f.ek[t] = *reinterpret_cast<const unsigned int*>(p.exps + w.rows[t] + 4 * g);
     }
     __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the work they are to overlap
@@ -548,11 +550,13 @@ struct Wave {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const char* vb = p.kv + (w.rows[t] + page_size) * (D * E);  // V lies page_size rows behind K
+      const unsigned int most = w.valid[t] > 0 ? w.valid[t] - 1 : 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r) {
+        const unsigned int row = 4 * g + r < most ? 4 * g + r : most;
 #pragma unroll
-        for (int h = 0; h < VH; ++h)
-          fetch<VB>(f.v[t][r][h], vb + r * (D * E) + h * (VB * 16) + (4 * g * (D * E) + c * VB));
+        for (int h = 0; h < VH; ++h) fetch<VB>(f.v[t][r][h], vb + h * (VB * 16) + (row * (D * E) + c * VB));
+      }
       if (DT == MI_DT_E4M3) f.ev[t] = *reinterpret_cast<const unsigned int*>(p.exps + w.rows[t] + page_size + 4 * g);
     }
     __builtin_amdgcn_sched_barrier(0);
