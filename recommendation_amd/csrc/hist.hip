@@ -436,7 +436,8 @@ struct Wave {
   static constexpr float SLACK = 8.f;
 
   f4v o[RT][VH][VE];
-  // l: a column of the second product whose "values" are all 1, so that every lane of a row holds the whole sum
+  // l: in 8 and 16 bits a column of the second product whose "values" are all 1, so that every lane of a row holds the
+  // whole sum; in f32, where that product takes four times as long, the lane's own positions until close()
   float m[RT];
   f4v l[RT];
   bf8v qf[RT][F32 ? 1 : NS];
@@ -698,7 +699,7 @@ struct Wave {
       // are multiplied by the value row's power of two, exactly, and their sum's column holds its inverse.
       if constexpr (F32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) l[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.f, w[i][e], l[i], 0, 0, 0);
+        for (int e = 0; e < 8; ++e) l[i][0] += w[i][e];
       } else {
         unsigned int pw[4];
 #pragma unroll
@@ -754,6 +755,17 @@ struct Wave {
             o[i][h][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, b), pf[i], o[i][h][j + 1], 0, 0, 0);
           }
         }
+    }
+  }
+
+  // f32: the four g hold the sums of their own positions
+  __device__ __forceinline__ void close() {
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        l[i][0] += __shfl_xor(l[i][0], 16, 64);
+        l[i][0] += __shfl_xor(l[i][0], 32, 64);
+      }
     }
   }
 
@@ -842,6 +854,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
     w.init(t, q_row_of<W::QE>(p, b, head, row, row < p.rows), row < p.rows, g);
   }
   w.walk(p, p.table + b * p.ld_table, 0, (unsigned int) len, W::CHUNK, head, lane);
+  w.close();
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int row = row0 + t * 16 + c;
@@ -957,6 +970,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
     const int32_t* table = p.table + (int64_t) b * p.ld_table;
     const unsigned int end = ue == u ? (unsigned int) len : ue * unit;
     if (row0 < p.rows) w.walk(p, table, ub * unit + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
+    w.close();
       // the waves that shared the positions of a row tile: halves fold together, lane by lane
     for (int half = CI >> 1; half > 0; half >>= 1) {
       const int slot = (ci - half) * a.NR + rt;  // < 2: half * NR <= 2
