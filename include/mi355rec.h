@@ -949,8 +949,9 @@ int mi_hist_read(const mi_hist_cache* cache, void* k, void* v, int dtype, int64_
 /* Attention of n_queries new tokens (or candidates) of every sequence over ALL lengths[b] positions of its history:
  *   out[b][t][h] = sum_j softmax_j(scale * <q[b][t][h], k_j>) v_j,   k_j, v_j of cache head h / (q_heads / n_heads).
  * Queries of one sequence do not see each other.  A row without a position of finite score gives zeros.  q, out:
- * f32 for an f32 cache, bf16 otherwise; sequence, token and head strides in elements, 16-byte aligned.  Sums and
- * softmax statistics in f32. */
+ * f32 for an f32 cache, bf16 otherwise; sequence, token and head strides in elements, 16-byte aligned; out may be q.
+ * Sums and softmax statistics in f32; weighted values are summed before they are divided, so values should stay below
+ * 2^100 in size (and an e4m3 cache's above 2^-100, where their weights would leave bf16's normal range). */
 size_t mi_hist_attn_workspace_bytes(const mi_hist_cache* cache, int64_t n_seqs, int n_queries, int q_heads, int table_width);
 int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q_seq, int64_t q_tok, int64_t q_head, int q_heads,
                  int n_queries, int64_t n_seqs, const int32_t* page_table, int64_t ld_table, int table_width,

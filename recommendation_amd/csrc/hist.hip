@@ -405,7 +405,12 @@ struct AttnArgs {
   int32_t* err;
 };
 
-// One wave's running state for 16 query rows of one cache head: o = sum_j 2^(s_j - m) v_j, l = sum_j 2^(s_j - m).
+// Waves on a SIMD, asked of the compiler (registers) and counted on when the work is cut.
+constexpr int split_waves(bool f32, int dim, int RT) {
+  return dim == 256 ? 1 : dim == 128 ? (f32 ? 3 - RT : 4 - RT) : dim == 64 ? (f32 ? 3 : 4) - (RT - 1) : 4 - (RT - 1);
+}
+
+// One wave's running state for RT tiles of 16 query rows of one cache head: o = sum_j 2^(s_j - m) v_j, l = sum_j 2^(s_j - m).
 //
 // Both products are matrix instructions whose operands come straight from memory.  Scores are formed transposed,
 // S^T = K Q^T (rows: 16 cached positions; columns: query rows): lane (g = lane / 16, c = lane % 16) then holds the
@@ -413,11 +418,9 @@ struct AttnArgs {
 // its right operand if its reduction index is read as "positions 4g..4g+3 of tile 0, then of tile 1".  Its left
 // operand takes output channels j of 16 lanes' 16-byte pieces of a V row, whatever those channels are called.  So no
 // score, probability or value crosses lanes; only the row maximum and sum do (over the four g).
-// Waves on a SIMD, asked of the compiler (registers) and counted on when the work is cut.
-constexpr int split_waves(bool f32, int dim, int RT) {
-  return dim == 256 ? 1 : dim == 128 ? (f32 ? 3 - RT : 4 - RT) : dim == 64 ? (f32 ? 3 : 4) - (RT - 1) : 4 - (RT - 1);
-}
-
+//
+// What bounds it: the cache's bytes (1 to 16 query rows a head: 6.2-6.7 TB/s over long histories), and from two row tiles
+// on the vector instructions (e4m3, 64 rows: 62 % of the issue slots).
 template <int DT, int D, int RT, bool STREAM>
 struct Wave {
   static constexpr bool F32 = DT == MI_DT_F32;
@@ -660,15 +663,7 @@ struct Wave {
     }
     float w[RT][8];
     bf8v pf[RT];
-    uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);  // bf16
-    if constexpr (DT == MI_DT_E4M3) {
-      unsigned int* po = &ones.x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // exponent field 254 - exps; dead positions (0 here) have weight 0
-        const unsigned int two = f.ev[e >> 1] >> (16 * (e & 1));
-        po[e] = 0x7f007f00u - (((two & 255u) << 7) | ((two & 0xff00u) << 15));
-      }
-    }
+    const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);  // bf16
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       float top = m[i];
@@ -696,22 +691,23 @@ struct Wave {
         for (int r = 0; r < 4; ++r) w[i][4 * t + r] = __builtin_amdgcn_exp2f(s[i][t][r] - base);
       // 8- and 16-bit caches: the weights enter the product as bf16 (off by half a step, 2^-8 of the weight at most, as
       // the output's own rounding is), and the sum they are divided by is that of the rounded weights.  In 8 bits they
-      // are multiplied by the value row's power of two, exactly, and their sum's column holds its inverse.
+      // then carry the value row's power of two, which changes no bit of them - but their sum does not: a row of zeros
+      // has the power 2^-126 and its weight all the same.
       if constexpr (F32) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) l[i][0] += w[i][e];
       } else {
-        unsigned int pw[4];
+        u4v pw;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (DT == MI_DT_E4M3)
+        for (int e = 0; e < 4; ++e) pw[e] = pack_bf16(w[i][2 * e], w[i][2 * e + 1]);
+        l[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, ones), __builtin_bit_cast(bf8v, pw), l[i], 0, 0, 0);
+        if constexpr (DT == MI_DT_E4M3) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
             pw[e] = pack_bf16(w[i][2 * e] * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1))) & 255u),
                               w[i][2 * e + 1] * pow2_bits((f.ev[e >> 1] >> (16 * (e & 1) + 8)) & 255u));
-          else
-            pw[e] = pack_bf16(w[i][2 * e], w[i][2 * e + 1]);
         }
-        pf[i] = __builtin_bit_cast(bf8v, make_uint4(pw[0], pw[1], pw[2], pw[3]));
-        l[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, ones), pf[i], l[i], 0, 0, 0);
+        pf[i] = __builtin_bit_cast(bf8v, pw);
       }
     }
     if constexpr (F32) {

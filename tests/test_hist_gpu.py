@@ -333,6 +333,32 @@ def test_attention_with_peaked_and_flat_scores(dev, cache):
     run_attn(dev, rng, cache, lens, 16, 2, 2, 1, 64, scale=-0.3, name='negative scale')
 
 
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('power', [None, -100, -60, 60, 90])
+def test_attention_over_rows_of_zeros_and_of_extreme_size(dev, cache, power):
+    """Value rows of zeros (their weights count all the same), and keys and values of very small or large size."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(17)
+    for lens in ([100, 7, 33], [700, 40, 3]):
+        c, table, lengths, t = filled(dev, rng, cache, lens, 16, 2, 64)
+        n = sum(lens)
+        offs = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int64, device=dev)
+        k, v = ops.hist_read(c, table, lengths, n, offsets=offs, dtype=torch.float32)
+        zero = torch.from_numpy(rng.random((n, 1, 1)) < 0.5).to(dev)
+        if power is None:
+            v = torch.where(zero, torch.zeros_like(v), v)
+            k = torch.where(torch.from_numpy(rng.random((n, 1, 1)) < 0.1).to(dev), torch.zeros_like(k), k)
+        else:
+            v = v * 2.0 ** power                               # exact in every type
+        ops.hist_write(c, k, v, table, lengths, offsets=offs)
+        dt = torch.float32 if cache == 'f32' else torch.bfloat16
+        q = torch.from_numpy(rng.standard_normal((3, 1, 4, 64))).to(dev, dt)
+        got = ops.hist_attn(c, q, table, lengths).double().cpu().numpy()
+        want, absv, size = oh.attention(values(c), q.double().cpu().numpy(), t, lens, 0.125, 16)
+        held("hist_attn %s rows of zeros / 2^%s, up to %d" % (cache, power, max(lens)),
+             (np.abs(got - want) / bound(cache, 64, max(lens), want, absv, size)).max(), 1.0)
+
+
 @pytest.mark.parametrize('cache', ['bf16', 'e4m3'])
 def test_strided_queries_shared_pages_and_table_views(dev, cache):
     """Queries as a slice of a fused projection, several sequences on the same pages, a page table that is a view."""
