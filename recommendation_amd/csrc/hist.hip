@@ -858,6 +858,75 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   }
 }
 
+// A workgroup's walk over positions first .. end-1 of one (sequence, cache head, group of NR * 16 * RT query rows): NR row
+// tiles side by side, the other waves share the positions (32 each in turn) and fold their sums in LDS, halves onto halves,
+// lane by lane the same rows and channels.  Afterwards the first NR waves hold the sums.
+template <typename W, int RT>
+struct FoldLds {
+  f4v o[2][RT * W::VH * W::VE][64];
+  float2 ml[2][RT][64];
+};
+template <typename W, int RT>
+__device__ __forceinline__ void walk_shared(W& w, FoldLds<W, RT>& lds, const AttnArgs& p, int NR, int64_t b, int head, int row0,
+                                            unsigned int first, unsigned int end, int wave, int lane) {
+  const int g = lane >> 4, c = lane & 15, rt = wave % NR, ci = wave / NR, CI = 4 / NR;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int row = row0 + t * 16 + c;
+    w.init(t, q_row_of<W::QE>(p, b, head, row, row < p.rows), row < p.rows, g);
+  }
+  if (row0 < p.rows) w.walk(p, p.table + b * p.ld_table, first + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
+  w.close();
+  for (int half = CI >> 1; half > 0; half >>= 1) {
+    const int slot = (ci - half) * NR + rt;  // < 2: half * NR <= 2
+    if (ci >= half && ci < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        lds.ml[slot][t][lane] = make_float2(w.m[t], w.l[t][0]);
+#pragma unroll
+        for (int i = 0; i < W::VH * W::VE; ++i) lds.o[slot][t * W::VH * W::VE + i][lane] = w.o[t][i / W::VE][i % W::VE];
+      }
+    }
+    __syncthreads();
+    if (ci < half) {
+      const int from = ci * NR + rt;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float2 ml = lds.ml[from][t][lane];
+        const Fold k = fold_of(w.m[t], ml.x);
+        w.m[t] = k.m;
+        w.l[t][0] = w.l[t][0] * k.a + ml.y * k.b;
+#pragma unroll
+        for (int i = 0; i < W::VH * W::VE; ++i)
+          w.o[t][i / W::VE][i % W::VE] = w.o[t][i / W::VE][i % W::VE] * k.a + lds.o[from][t * W::VH * W::VE + i][lane] * k.b;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Histories of a thousand positions at most: a workgroup to every (sequence, head, group), nothing is cut or joined.
+template <int DT, int D, int RT, bool STREAM>
+__global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist_attn_medium_kernel(AttnArgs p, int NR, int NG) {
+  typedef Wave<DT, D, RT, STREAM> W;
+  __shared__ FoldLds<W, RT> lds;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned int HG = (unsigned int) (p.H * NG), b = blockIdx.x / HG, pair = blockIdx.x - b * HG;
+  const int head = (int) (pair / (unsigned int) NG), grp = (int) (pair - (unsigned int) head * NG);
+  const int64_t len = clamped_length(p, scalar_load(p.lengths + b), pair == 0 && threadIdx.x == 0);
+  const int row0 = (grp * NR + wave % NR) * 16 * RT;
+  W w;
+  walk_shared(w, lds, p, NR, b, head, row0, 0, (unsigned int) len, wave, lane);
+  if (wave < NR) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = row0 + t * 16 + c;
+      if (row < p.rows) w.store(t, out_row_of<W::QE>(p, b, head, row), g);
+    }
+  }
+}
+
 // Long histories: the call's work is cut into equal runs of units, a unit being UNIT positions of one (sequence, cache
 // head, group of query rows), sequences slowest; a workgroup walks its run.  A run that begins or ends inside a
 // (sequence, head, group) leaves an unnormalised part, which the joining launch adds up.  The cut goes by the lengths
@@ -887,8 +956,7 @@ __device__ __forceinline__ unsigned int units_of(int64_t len, unsigned int unit)
 template <int DT, int D, int RT, bool STREAM>
 __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist_attn_split_kernel(AttnArgs p, SplitArgs a) {
   typedef Wave<DT, D, RT, STREAM> W;
-  __shared__ f4v lo[2][RT * W::VH * W::VE][64];
-  __shared__ float2 lml[2][RT][64];
+  __shared__ FoldLds<W, RT> lds;
   __shared__ unsigned int wave_sum[4];
   __shared__ unsigned int found[2];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -945,7 +1013,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   __syncthreads();
   if (x0 >= total) return;
 
-  const int rt = wave % a.NR, ci = wave / a.NR, CI = 4 / a.NR;
+  const int rt = wave % a.NR, ci = wave / a.NR;
   const int group_rows = a.NR * 16 * RT;
   unsigned int b = __builtin_amdgcn_readfirstlane(found[0]);
   unsigned int start = __builtin_amdgcn_readfirstlane(found[1]);
@@ -958,42 +1026,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
     const unsigned int ue = ub + (x1 - x) < u ? ub + (x1 - x) : u;
     const int row0 = (grp * a.NR + rt) * 16 * RT;
     W w;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int row = row0 + t * 16 + c;
-      w.init(t, q_row_of<W::QE>(p, b, head, row, row < p.rows), row < p.rows, g);
-    }
-    const int32_t* table = p.table + (int64_t) b * p.ld_table;
-    const unsigned int end = ue == u ? (unsigned int) len : ue * unit;
-    if (row0 < p.rows) w.walk(p, table, ub * unit + ci * W::CHUNK, end, CI * W::CHUNK, head, lane);
-    w.close();
-      // the waves that shared the positions of a row tile: halves fold together, lane by lane
-    for (int half = CI >> 1; half > 0; half >>= 1) {
-      const int slot = (ci - half) * a.NR + rt;  // < 2: half * NR <= 2
-      if (ci >= half && ci < 2 * half) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          lml[slot][t][lane] = make_float2(w.m[t], w.l[t][0]);
-#pragma unroll
-          for (int i = 0; i < W::VH * W::VE; ++i) lo[slot][t * W::VH * W::VE + i][lane] = w.o[t][i / W::VE][i % W::VE];
-        }
-      }
-      __syncthreads();
-      if (ci < half) {
-        const int from = ci * a.NR + rt;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const float2 ml = lml[from][t][lane];
-          const Fold k = fold_of(w.m[t], ml.x);
-          w.m[t] = k.m;
-          w.l[t][0] = w.l[t][0] * k.a + ml.y * k.b;
-#pragma unroll
-          for (int i = 0; i < W::VH * W::VE; ++i)
-            w.o[t][i / W::VE][i % W::VE] = w.o[t][i / W::VE][i % W::VE] * k.a + lo[from][t * W::VH * W::VE + i][lane] * k.b;
-        }
-      }
-      __syncthreads();
-    }
+    walk_shared(w, lds, p, a.NR, b, head, row0, ub * unit, ue == u ? (unsigned int) len : ue * unit, wave, lane);
     if (ci == 0) {
       const bool whole = ub == 0 && ue == u;
       const int64_t part = ((int64_t) (ub == 0 ? gridDim.x : 0) + blockIdx.x) * a.slot_rows - grp * group_rows;
@@ -1119,9 +1152,11 @@ __global__ __launch_bounds__(JOIN_THREADS) void hist_attn_join_kernel(AttnArgs p
                      __builtin_amdgcn_readfirstlane(first + (__ffsll((unsigned long long) todo) - 1) * subs), lacc, lml);
 }
 
+constexpr int64_t SHORT_ROOM = 256, MEDIUM_ROOM = 1024;
+
 // How a call is run; the same on every call of the same sizes.
 struct AttnPlan {
-  bool short_rows;
+  bool short_rows, medium;
   int RT, NR, NG, blocks, slot_rows;
   size_t parts_bytes, ml_bytes, bytes;
 };
@@ -1133,11 +1168,13 @@ AttnPlan plan_attn(int dtype, int dim, int H, int page_size, int64_t n_seqs, int
   const int64_t tiles = mi_cdiv(rows, 16 * q.RT);
   q.NR = tiles >= 3 ? 4 : (int) tiles;
   q.NG = (int) mi_cdiv(tiles, q.NR);
-  q.short_rows = room <= 256;
-  const int64_t most = n_seqs * H * q.NG * mi_cdiv(room, UNIT);
+  q.short_rows = room <= SHORT_ROOM;
+  const int64_t pairs = n_seqs * H * q.NG, most = pairs * mi_cdiv(room, UNIT);
   const int64_t resident = 256 * split_waves(dtype == MI_DT_F32, dim, q.RT);
   q.blocks = (int) (most < resident ? most : resident);
-  if (!q.short_rows) {
+  q.medium = !q.short_rows && room <= MEDIUM_ROOM && pairs <= (1 << 23);
+  if (q.medium) q.blocks = (int) pairs;
+  if (!q.short_rows && !q.medium) {
     const int64_t group_rows = q.NR * 16 * q.RT;
     q.slot_rows = (int) (rows < group_rows ? rows : group_rows);
     const size_t part_rows = (size_t) q.blocks * 2 * q.slot_rows;
@@ -1160,6 +1197,12 @@ int launch_short(const AttnArgs& p, const AttnPlan& q, hipStream_t s) {
 
 template <int DT, int D, bool STREAM>
 int launch_split(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) {
+  if (q.medium) {
+    if (q.RT == 2) hist_attn_medium_kernel<DT, D, D <= 128 ? 2 : 1, STREAM><<<q.blocks, 256, 0, s>>>(p, q.NR, q.NG);
+    else hist_attn_medium_kernel<DT, D, 1, STREAM><<<q.blocks, 256, 0, s>>>(p, q.NR, q.NG);
+    MI_LAUNCH_CHECK();
+    return MI_OK;
+  }
   SplitArgs a = {};
   a.NR = q.NR;
   a.NG = q.NG;

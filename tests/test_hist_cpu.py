@@ -128,17 +128,17 @@ def test_bad_attention_calls_are_refused():
 
 
 def test_attention_workspace_is_checked():
-    """Histories of up to 256 positions need none; beyond, what mi_hist_attn_workspace_bytes says."""
+    """Page tables of up to 1024 positions need none; beyond, what mi_hist_attn_workspace_bytes says."""
     from recommendation_amd import _lib
     lib = _lib.load()
     c = _cache()
     need = lambda **kw: lib.mi_hist_attn_workspace_bytes(ctypes.byref(_cache(**kw.pop('cache', {}))), kw.pop('seqs', 4), kw.pop('tokens', 1),
-                                                         kw.pop('heads', 2), kw.pop('width', 17))
-    assert need(width=16) == 0 and need() > 0
+                                                         kw.pop('heads', 2), kw.pop('width', 65))
+    assert need(width=16) == need(width=64) == 0 and need() > 0
     assert need(seqs=0) == need(tokens=0) == need(heads=3) == need(width=0) == need(cache=dict(dim=48)) == 0
     assert need(seqs=4096, width=4096) < 1 << 26
 
-    def rc(ws, ws_bytes, width=17, seqs=4, ld=100000000, tokens=1):
+    def rc(ws, ws_bytes, width=65, seqs=4, ld=100000000, tokens=1):
         code = lib.mi_hist_attn(ctypes.byref(c), 4096, 128, 128, 64, 2, tokens, seqs, 4096, ld, width, 4096, 0.1, 4096, 128, 128,
                                 64, ws, ws_bytes, None, None)
         return code, lib.mi_last_error().decode()

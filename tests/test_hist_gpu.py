@@ -237,10 +237,12 @@ EDGES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 63, 64, 65, 100, 127, 128, 129
 
 @pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
 @pytest.mark.parametrize('dim', [32, 64, 128, 256])
-def test_attention_at_every_edge_of_tile_and_page(dev, cache, dim):
+@pytest.mark.parametrize('room', [256, 1024, 2048])
+def test_attention_at_every_edge_of_tile_and_page(dev, cache, dim, room):
+    """A wave, a workgroup and a run of the cut to each history: chosen by what the page table has room for."""
     rng = np.random.default_rng(dim)
     for page, heads, group, tokens in ((16, 1, 1, 1), (64, 2, 4, 1), (32, 3, 5, 2), (128, 1, 7, 5)):
-        run_attn(dev, rng, cache, EDGES, page, heads, group, tokens, dim)
+        run_attn(dev, rng, cache, EDGES, page, heads, group, tokens, dim, width=room // page, name='room %d' % room)
 
 
 @pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
@@ -268,7 +270,9 @@ def test_attention_of_many_uneven_histories(dev, cache):
     lens = rng.integers(0, 600, size=700)
     lens[100:160] = 0
     lens[200:400] = rng.integers(-3, 3, size=200)
-    lens[-1], lens[0] = 3001, 1
+    lens[0] = 1
+    run_attn(dev, rng, cache, lens.tolist(), 16, 1, 2, 1, 32)
+    lens[-1] = 3001
     run_attn(dev, rng, cache, lens.tolist(), 16, 1, 2, 1, 32)
 
 
@@ -276,9 +280,14 @@ def test_attention_of_many_uneven_histories(dev, cache):
 @pytest.mark.parametrize('dim', [32, 64, 128, 256])
 def test_pools_beyond_the_last_level_cache(dev, cache, dim):
     """A pool of more than 256 MB is read past the caches; same sums, bit for bit, as over the same pages in a small one."""
-    from recommendation_amd import ops
     rng = np.random.default_rng(dim + 1)
-    page, heads, lens = 64, 2, [700, 0, 1, 1500]
+    page, heads = 64, 2
+    for lens in ([100, 0, 1, 150], [700, 0, 1, 90], [700, 0, 1, 1500]):
+        pool_beyond(dev, rng, cache, dim, page, heads, lens)
+
+
+def pool_beyond(dev, rng, cache, dim, page, heads, lens):
+    from recommendation_amd import ops
     c, table, lengths, t = filled(dev, rng, cache, lens, page, heads, dim)
     per_page = heads * 2 * page * dim * c.kv.element_size()
     n_pages = (300 << 20) // per_page + c.n_pages
@@ -385,11 +394,12 @@ def test_strided_queries_shared_pages_and_table_views(dev, cache):
 
 
 @pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
-def test_bad_pages_are_absent_and_reported(dev, cache):
+@pytest.mark.parametrize('width', [63, 70])
+def test_bad_pages_are_absent_and_reported(dev, cache, width):
     from recommendation_amd import ops
     rng = np.random.default_rng(21)
     lens = [100, 1000, 64, 40]
-    c, table, lengths, t = filled(dev, rng, cache, lens, 16, 2, 64, width=63)
+    c, table, lengths, t = filled(dev, rng, cache, lens, 16, 2, 64, width=width)
     t = t.copy()
     t[0, 2], t[0, 6], t[1, 5], t[1, 30:34] = -1, c.n_pages, 1 << 30, -7
     t[3, :] = -1                                                             # no page at all: zeros
@@ -533,7 +543,7 @@ def test_captured_attention_over_long_histories(dev):
 def test_the_result_may_replace_the_queries(dev):
     from recommendation_amd import ops
     rng = np.random.default_rng(15)
-    for lens in ([50, 3, 0], [4000, 70, 900]):
+    for lens in ([50, 3, 0], [600, 3, 0], [4000, 70, 900]):
         c, table, lengths, t = filled(dev, rng, 'e4m3', lens, 16, 2, 64)
         q = torch.from_numpy(rng.standard_normal((3, 20, 6, 64))).to(dev, torch.bfloat16)
         want = ops.hist_attn(c, q, table, lengths)
