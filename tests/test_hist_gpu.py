@@ -134,6 +134,46 @@ def test_write_and_read_are_exact(dev, cache, given, dim, heads, page):
     assert err.item() == 0
 
 
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_rows_of_any_stride_and_table_views(dev, cache):
+    """Heads in front of tokens, K and V of one fused projection, outputs with gaps, a page table inside a wider one; the same
+    calls captured into a graph."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(23)
+    page, heads, dim, lens = 16, 3, 64, [40, 9, 100]
+    n = sum(lens)
+    dt = torch.float32 if cache == 'f32' else torch.bfloat16
+    t = tables(rng, lens, page, 7, 20)
+    wide = torch.full((3, 16), -1, dtype=torch.int32, device=dev)
+    wide[:, 5:12] = torch.from_numpy(t).to(dev)
+    table, lengths = wide[:, 5:12], torch.tensor(lens, dtype=torch.int32, device=dev)
+    offs = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int64, device=dev)
+    fused = torch.from_numpy(rng.standard_normal((n, 9 * dim + 32))).to(dev, dt)
+    k = fused[:, 32:32 + heads * dim].view(n, heads, dim)
+    v = torch.from_numpy(rng.standard_normal((heads, n, dim))).to(dev, dt).transpose(0, 1)
+    plain, c = poisoned(dev, cache, 20, page, heads, dim), poisoned(dev, cache, 20, page, heads, dim)
+    ops.hist_write(plain, k.contiguous(), v.contiguous(), table.contiguous(), lengths, offsets=offs)
+    out = torch.full((n, 2, heads, dim + 16), 5.0, dtype=dt, device=dev)
+    pair = (out[:, 0, :, :dim], out[:, 1, :, 16:])
+    ops.hist_read(plain, table, lengths, offsets=offs, out=pair)             # also outside capture: nothing is set up
+    first = out.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.hist_write(c, k, v, table, lengths, offsets=offs)
+        ops.hist_read(c, table, lengths, offsets=offs, out=pair)
+    for _ in range(3):
+        c.kv.view(torch.uint8).fill_(0x7f)
+        out.fill_(5.0)
+        g.replay()
+        torch.cuda.synchronize()
+        np.testing.assert_array_equal(values(c)[t[t >= 0]], np.where(np.isnan(values(plain)[t[t >= 0]]),
+                                                                     values(c)[t[t >= 0]], values(plain)[t[t >= 0]]))
+        assert torch.equal(out, first)
+    k1, v1 = ops.hist_read(plain, table, lengths, n, offsets=offs, dtype=dt)
+    assert torch.equal(pair[0], k1) and torch.equal(pair[1], v1)
+    assert bool((out[:, 0, :, dim:] == 5.0).all()) and bool((out[:, 1, :, :16] == 5.0).all())
+
+
 def test_rows_without_a_place(dev):
     """Lengths shorter than the rows given, padded sequences, bad pages and histories beyond the table."""
     from recommendation_amd import ops
