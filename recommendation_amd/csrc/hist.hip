@@ -1001,7 +1001,7 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   const unsigned int x0 = blockIdx.x * run, x1 = x0 + run < total ? x0 + run : total;
   if (x0 < total && before * HG <= x0 && x0 < (before + mine) * HG) {
     unsigned int b = s0;
-    for (;; ++b) {
+    for (; b + 1 < s1; ++b) {
       const unsigned int u = units_of(clamped_length(p, p.lengths[b], false), unit);
       if (x0 < (before + u) * HG) break;
       before += u;
@@ -1018,10 +1018,11 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
   unsigned int b = __builtin_amdgcn_readfirstlane(found[0]);
   unsigned int start = __builtin_amdgcn_readfirstlane(found[1]);
   unsigned int x = x0;
-  while (x < x1) {
+  while (x < x1 && b < n_seqs) {
     const int64_t len = clamped_length(p, scalar_load(p.lengths + b), false);
     const unsigned int u = units_of(len, unit);
     const unsigned int rem = x - start, pair = rem / u, ub = rem - pair * u;
+    if (pair >= HG) break;  // lengths that change under the launch give nonsense, but no access out of bounds
     const int head = (int) (pair / (unsigned int) a.NG), grp = (int) (pair - (unsigned int) head * a.NG);
     const unsigned int ue = ub + (x1 - x) < u ? ub + (x1 - x) : u;
     const int row0 = (grp * a.NR + rt) * 16 * RT;
@@ -1038,8 +1039,10 @@ __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist
           else w.store_part(t, a.parts + (part + row) * D, a.part_ml + part + row, g);
         }
       }
-      if (threadIdx.x == 0 && ub == 0 && ue < u)
-        a.meta[blockIdx.x] = make_int4((int) b, (int) pair, (int) ((x + u - 1) / run), 0);
+      if (threadIdx.x == 0 && ub == 0 && ue < u) {
+        const unsigned int last = (x + u - 1) / run;
+        a.meta[blockIdx.x] = make_int4((int) b, (int) pair, (int) (last < gridDim.x ? last : gridDim.x - 1), 0);
+      }
     }
     x += ue - ub;
     if (ue == u && pair + 1 == HG) {

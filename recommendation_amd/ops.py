@@ -1038,6 +1038,7 @@ class HistCache(object):
                                  n_pages=self.n_pages, n_heads=self.n_heads, page_size=self.page_size, dim=self.dim,
                                  dtype=self._DTYPES[dtype])
         self._ref = ctypes.byref(self.c)
+        self._scale = self.dim ** -0.5
 
     def ref(self):
         return self._ref
@@ -1060,13 +1061,17 @@ def _hist_common(what, cache, page_table, lengths, offsets, err, x, y):
     if len(shape) != 2 or page_table.dtype is not torch.int32 or shape[1] < 1 or (stride[1] != 1 and shape[1] > 1):
         raise MiError("%s: page_table must be int32 [sequences, pages] with contiguous rows" % what)
     n = shape[0]
-    if lengths.shape != (n,) or lengths.dtype is not torch.int32 or not lengths.is_contiguous():
+    if lengths.dim() != 1 or lengths.numel() != n or lengths.dtype is not torch.int32 or not lengths.is_contiguous():
         raise MiError("%s: lengths must be contiguous int32 [%d]" % (what, n))
     if offsets is not None and (offsets.shape != (n + 1,) or offsets.dtype is not torch.int64 or not offsets.is_contiguous()):
         raise MiError("%s: offsets must be contiguous int64 [%d]" % (what, n + 1))
     if err is not None and (err.dtype is not torch.int32 or err.numel() < 1):
         raise MiError("%s: err must be an int32 error word (new_error_word)" % what)
     return n, shape[1], stride[0]
+
+
+def _hist_stream(dev):
+    return _RAW_STREAM(dev) if _RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _hist_rows_call(name, what, cache, k, v, page_table, lengths, offsets, err):
@@ -1087,7 +1092,7 @@ def _hist_rows_call(name, what, cache, k, v, page_table, lengths, offsets, err):
         ks, vs = ([0 if shape[d] <= 1 else st[d] for d in range(2)] for st in (ks, vs))
     _lib.call(name, cache._ref, k.data_ptr(), v.data_ptr(), MI_DT_BF16 if dtype is torch.bfloat16 else MI_DT_F32, ks[0], ks[1],
               vs[0], vs[1], rows, offsets.data_ptr() if offsets is not None else None, n, page_table.data_ptr(), ld_table,
-              width, lengths.data_ptr(), err.data_ptr() if err is not None else None, _stream())
+              width, lengths.data_ptr(), err.data_ptr() if err is not None else None, _hist_stream(cache._index))
 
 
 def hist_write(cache, k, v, page_table, lengths, offsets=None, err=None):
@@ -1105,7 +1110,7 @@ def hist_read(cache, page_table, lengths, n_rows=None, offsets=None, dtype=torch
     if out is None:
         if n_rows is None:
             raise MiError("hist_read: give n_rows or out")
-        k = torch.empty((int(n_rows), cache.n_heads, cache.dim), dtype=dtype, device=cache.kv.device)
+        k = cache.kv.new_empty((int(n_rows), cache.n_heads, cache.dim), dtype=dtype)
         out = k, torch.empty_like(k)
     elif n_rows is not None and out[0].shape[0] != n_rows:
         raise MiError("hist_read: out holds %d rows, n_rows says %d" % (out[0].shape[0], n_rows))
@@ -1143,9 +1148,9 @@ def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
         sizes = (n, tokens, shape[-2])
         qs, os_ = ([st[d] if sizes[d] > 1 else 0 for d in range(3)] for st in (qs, os_))
     ws_bytes = _lib.load().mi_hist_attn_workspace_bytes(cache._ref, n, tokens, shape[-2], width)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     _lib.call('mi_hist_attn', cache._ref, q.data_ptr(), qs[0], qs[1], qs[2], shape[-2], tokens, n, page_table.data_ptr(),
-              ld_table, width, lengths.data_ptr(), dim ** -0.5 if scale is None else scale, out.data_ptr(), os_[0], os_[1],
+              ld_table, width, lengths.data_ptr(), cache._scale if scale is None else scale, out.data_ptr(), os_[0], os_[1],
               os_[2], ws.data_ptr() if ws is not None else None, ws_bytes, err.data_ptr() if err is not None else None,
-              _stream())
+              _hist_stream(cache._index))
     return out
