@@ -1279,6 +1279,9 @@ bool aligned16(const void* p, int elem, int64_t a, int64_t b, int64_t c = 0) {
   return (((uintptr_t) p | (uintptr_t) (a * elem) | (uintptr_t) (b * elem) | (uintptr_t) (c * elem)) & 15) == 0;
 }
 
+// results: two entries of a dimension must not share memory (an expanded tensor), their rows would be written in no order
+bool apart(int64_t n, int64_t stride, int dim) { return n <= 1 || stride >= dim; }
+
 int rows_call(const char* who, bool read, const mi_hist_cache* cache, const void* k, const void* v, int dtype, int64_t k_row,
               int64_t k_head, int64_t v_row, int64_t v_head, int64_t n_rows, const int64_t* offsets, int64_t n_seqs,
               const int32_t* table, int64_t ld_table, int width, const int32_t* lengths, int32_t* err, void* stream) {
@@ -1290,6 +1293,9 @@ int rows_call(const char* who, bool read, const mi_hist_cache* cache, const void
   MI_REQUIRE(k && v, "%s: null rows", who);
   MI_REQUIRE(aligned16(k, dtype == MI_DT_F32 ? 4 : 2, k_row, k_head) && aligned16(v, dtype == MI_DT_F32 ? 4 : 2, v_row, v_head),
              "%s: rows must start on 16-byte boundaries", who);
+  MI_REQUIRE(!read || (apart(n_rows, k_row, cache->dim) && apart(n_rows, v_row, cache->dim) &&
+                       apart(cache->n_heads, k_head, cache->dim) && apart(cache->n_heads, v_head, cache->dim)),
+             "%s: the rows to be filled overlap", who);
   MI_REQUIRE(offsets || n_rows % n_seqs == 0, "%s: %lld rows do not divide among %lld sequences", who, (long long) n_rows,
              (long long) n_seqs);
   if (n_rows * 2 * cache->n_heads > (int64_t) INT32_MAX) {
@@ -1379,6 +1385,8 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
   const int qe = cache->dtype == MI_DT_F32 ? 4 : 2;
   MI_REQUIRE(aligned16(q, qe, q_seq, q_tok, q_head) && aligned16(out, qe, out_seq, out_tok, out_head),
              "mi_hist_attn: the rows of q and out must start on 16-byte boundaries");
+  MI_REQUIRE(apart(n_seqs, out_seq, cache->dim) && apart(n_queries, out_tok, cache->dim) && apart(q_heads, out_head, cache->dim),
+             "mi_hist_attn: the rows of out overlap");
   AttnArgs p = {};
   p.kv = (const char*) cache->kv;
   p.exps = (const uint8_t*) cache->exps;

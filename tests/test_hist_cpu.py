@@ -165,3 +165,35 @@ def test_host_tensors_are_refused():
             ops.HistCache(device='cpu', **args)
     with pytest.raises(TypeError, match='HistCache'):
         ops.HistCache(4, 16, 2, 64, dtype=torch.float16, device='cpu')
+
+
+def test_results_that_overlap_are_refused():
+    """An expanded result (a stride of zero, or below a row's length) would take several rows in one place, in no order.
+    Inputs may be expanded, and the stride of a dimension of one entry says nothing."""
+    from recommendation_amd import _lib
+    lib = _lib.load()
+    one = _cache(n_heads=1)
+
+    def read(strides, c=None, n=4, offsets=4096):
+        code = lib.mi_hist_read(ctypes.byref(c or _cache()), 4096, 4096, 1, *strides, n, offsets, 4, 4096, 2, 2, 4096, None, None)
+        return code, lib.mi_last_error().decode()
+
+    for strides in ((0, 64, 128, 64), (128, 64, 0, 64), (128, 0, 128, 64), (128, 64, 128, 0), (56, 64, 128, 64), (-128, 64, 128, 64)):
+        code, msg = read(strides)
+        assert code == -1 and 'overlap' in msg, (strides, msg)
+    # one row, one head: those strides are not looked at; the call goes on to the next check (rows of one call)
+    for strides, c in (((128, 0, 128, 0), one), ((64, 0, 64, 0), one)):
+        code, msg = read(strides, c, n=1 << 30)
+        assert code == -4 and 'in one call' in msg, (strides, code, msg)
+
+    def attn(os_, tokens=2, seqs=4, heads=2, width=65):
+        code = lib.mi_hist_attn(ctypes.byref(_cache()), 4096, 0, 0, 0, heads, tokens, seqs, 4096, width, width, 4096, 0.1, 4096,
+                                *os_, None, 0, None, None)
+        return code, lib.mi_last_error().decode()
+
+    for os_ in ((0, 128, 64), (256, 0, 64), (256, 128, 0), (256, 128, 32)):
+        code, msg = attn(os_)
+        assert code == -1 and 'overlap' in msg, (os_, msg)
+    for os_, kw in (((256, 128, 64), {}), ((128, 0, 64), dict(tokens=1)), ((0, 128, 64), dict(seqs=1))):
+        code, msg = attn(os_, **kw)                               # past that check: the workspace is the next
+        assert code == -3 and 'workspace' in msg, (os_, kw, msg)
