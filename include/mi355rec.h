@@ -941,7 +941,8 @@ int mi_hist_write(const mi_hist_cache* cache, const void* k, const void* v, int 
                   int32_t* err, void* stream);
 
 /* The mirror image: k, v (f32 or bf16) = the newest positions, packed by the same rule.  Rows nobody owns are left as
- * they are; rows without a place in the cache (in front of position 0, bad page) become zeros.  Rows must not overlap. */
+ * they are; rows without a place in the cache (in front of position 0, bad page) become zeros.  The rows of k and v must
+ * not overlap, each other's neither: in each of the two a stride reaches over all that lies inside it. */
 int mi_hist_read(const mi_hist_cache* cache, void* k, void* v, int dtype, int64_t k_row, int64_t k_head, int64_t v_row,
                  int64_t v_head, int64_t n_rows, const int64_t* offsets, int64_t n_seqs, const int32_t* page_table,
                  int64_t ld_table, int table_width, const int32_t* lengths, int32_t* err, void* stream);
@@ -949,8 +950,8 @@ int mi_hist_read(const mi_hist_cache* cache, void* k, void* v, int dtype, int64_
 /* Attention of n_queries new tokens (or candidates) of every sequence over ALL lengths[b] positions of its history:
  *   out[b][t][h] = sum_j softmax_j(scale * <q[b][t][h], k_j>) v_j,   k_j, v_j of cache head h / (q_heads / n_heads).
  * Queries of one sequence do not see each other.  A row without a position of finite score gives zeros.  q, out:
- * f32 for an f32 cache, bf16 otherwise; sequence, token and head strides in elements, 16-byte aligned; out may be q,
- * and its own rows must not overlap.
+ * f32 for an f32 cache, bf16 otherwise; sequence, token and head strides in elements, 16-byte aligned.  out may be q
+ * (the same rows in the same places) and must not overlap it otherwise; its own rows must not overlap, as in a read.
  * Sums and softmax statistics in f32; weighted values are summed before they are divided, so values should stay below
  * 2^100 in size (and an e4m3 cache's above 2^-100, where their weights would leave bf16's normal range). */
 size_t mi_hist_attn_workspace_bytes(const mi_hist_cache* cache, int64_t n_seqs, int n_queries, int q_heads, int table_width);

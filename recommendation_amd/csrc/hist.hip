@@ -1279,8 +1279,64 @@ bool aligned16(const void* p, int elem, int64_t a, int64_t b, int64_t c = 0) {
   return (((uintptr_t) p | (uintptr_t) (a * elem) | (uintptr_t) (b * elem) | (uintptr_t) (c * elem)) & 15) == 0;
 }
 
-// results: two entries of a dimension must not share memory (an expanded tensor), their rows would be written in no order
-bool apart(int64_t n, int64_t stride, int dim) { return n <= 1 || stride >= dim; }
+// Rows of `dim` elements as a call names them, for the checks of what it writes.  Dimensions of one entry and of stride 0
+// are left out and strides taken as positive, neither changes which memory the rows cover; smallest stride first.
+struct RowSet {
+  __int128 first;  // of the lowest element, in bytes
+  int elem, dim, n_dims;
+  struct { __int128 n, stride; } d[3];
+  bool repeats;    // a stride of 0 over several entries
+
+  RowSet(const void* p, int elem, int dim) : first((__int128) (uintptr_t) p), elem(elem), dim(dim), n_dims(0), repeats(false) {}
+  RowSet& over(int64_t n, int64_t stride) {
+    if (n <= 1) return *this;
+    if (stride == 0) {
+      repeats = true;
+      return *this;
+    }
+    __int128 s = stride;
+    if (s < 0) {
+      first += (n - 1) * s * elem;
+      s = -s;
+    }
+    int i = n_dims++;
+    for (; i > 0 && d[i - 1].stride > s; --i) d[i] = d[i - 1];
+    d[i].n = n;
+    d[i].stride = s;
+    return *this;
+  }
+  __int128 extent(int levels) const {  // elements from the first to behind the last, over the inner `levels` dimensions
+    __int128 e = dim;
+    for (int i = 0; i < levels; ++i) e += (d[i].n - 1) * d[i].stride;
+    return e;
+  }
+  // No two rows share memory: every stride reaches over all that lies inside it.  (Other sets without an overlap, strides of
+  // 2 and 3 rows over two entries each, do not count as apart.)
+  bool apart() const {
+    if (repeats) return false;
+    for (int i = 0; i < n_dims; ++i)
+      if (d[i].stride < extent(i)) return false;
+    return true;
+  }
+  // May share memory: exactly so where the two differ in their start alone (or, from some dimension inwards, lie in separate
+  // stretches), otherwise by their whole stretches.  `ahead`: elements from this set's first to the other's.
+  bool meets(const RowSet& o) const {
+    const __int128 bytes = o.first - first;
+    if (bytes % elem) return first < o.first + o.extent(o.n_dims) * elem && o.first < first + extent(n_dims) * elem;
+    return meets(o, n_dims, o.n_dims, bytes / elem);
+  }
+  bool meets(const RowSet& o, int a, int b, __int128 ahead) const {
+    if (ahead >= extent(a) || -ahead >= o.extent(b)) return false;
+    if (a == 0 && b == 0) return true;
+    if (a == 0 || b == 0 || d[a - 1].n != o.d[b - 1].n || d[a - 1].stride != o.d[b - 1].stride) return true;
+    const __int128 n = d[a - 1].n, s = d[a - 1].stride;
+    if (extent(a - 1) > s || o.extent(b - 1) > s) return true;
+    const __int128 t = -ahead / s;  // entries t apart come within a stride of each other, and those beside
+    for (__int128 i = t - 1; i <= t + 1; ++i)
+      if (i > -n && i < n && meets(o, a - 1, b - 1, ahead + i * s)) return true;
+    return false;
+  }
+};
 
 int rows_call(const char* who, bool read, const mi_hist_cache* cache, const void* k, const void* v, int dtype, int64_t k_row,
               int64_t k_head, int64_t v_row, int64_t v_head, int64_t n_rows, const int64_t* offsets, int64_t n_seqs,
@@ -1293,14 +1349,17 @@ int rows_call(const char* who, bool read, const mi_hist_cache* cache, const void
   MI_REQUIRE(k && v, "%s: null rows", who);
   MI_REQUIRE(aligned16(k, dtype == MI_DT_F32 ? 4 : 2, k_row, k_head) && aligned16(v, dtype == MI_DT_F32 ? 4 : 2, v_row, v_head),
              "%s: rows must start on 16-byte boundaries", who);
-  MI_REQUIRE(!read || (apart(n_rows, k_row, cache->dim) && apart(n_rows, v_row, cache->dim) &&
-                       apart(cache->n_heads, k_head, cache->dim) && apart(cache->n_heads, v_head, cache->dim)),
-             "%s: the rows to be filled overlap", who);
   MI_REQUIRE(offsets || n_rows % n_seqs == 0, "%s: %lld rows do not divide among %lld sequences", who, (long long) n_rows,
              (long long) n_seqs);
   if (n_rows * 2 * cache->n_heads > (int64_t) INT32_MAX) {
     mi_set_error("%s: %lld rows of %d heads in one call (at most 2^31-1 rows of K and V)", who, (long long) n_rows, cache->n_heads);
     return MI_ERR_UNSUPPORTED;
+  }
+  if (read) {  // rows that share memory would be written in no order
+    const int e = dtype == MI_DT_F32 ? 4 : 2;
+    const RowSet ks = RowSet(k, e, cache->dim).over(n_rows, k_row).over(cache->n_heads, k_head);
+    const RowSet vs = RowSet(v, e, cache->dim).over(n_rows, v_row).over(cache->n_heads, v_head);
+    MI_REQUIRE(ks.apart() && vs.apart() && !ks.meets(vs), "%s: the rows to be filled overlap", who);
   }
   RowArgs p = {};
   p.kv = (char*) cache->kv;
@@ -1385,8 +1444,6 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
   const int qe = cache->dtype == MI_DT_F32 ? 4 : 2;
   MI_REQUIRE(aligned16(q, qe, q_seq, q_tok, q_head) && aligned16(out, qe, out_seq, out_tok, out_head),
              "mi_hist_attn: the rows of q and out must start on 16-byte boundaries");
-  MI_REQUIRE(apart(n_seqs, out_seq, cache->dim) && apart(n_queries, out_tok, cache->dim) && apart(q_heads, out_head, cache->dim),
-             "mi_hist_attn: the rows of out overlap");
   AttnArgs p = {};
   p.kv = (const char*) cache->kv;
   p.exps = (const uint8_t*) cache->exps;
@@ -1421,6 +1478,8 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
                  (long long) tiles, table_width);
     return MI_ERR_UNSUPPORTED;
   }
+  const RowSet outs = RowSet(out, qe, cache->dim).over(n_seqs, out_seq).over(n_queries, out_tok).over(q_heads, out_head);
+  MI_REQUIRE(outs.apart(), "mi_hist_attn: the rows of out overlap");
   if (plan.bytes) {
     MI_REQUIRE(((uintptr_t) workspace & 15) == 0, "mi_hist_attn: the workspace must be 16-byte aligned");
     if (!workspace || workspace_bytes < plan.bytes) {
@@ -1428,6 +1487,11 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
       return MI_ERR_WORKSPACE;
     }
   }
+  // a row of out that is another row of q would be written while that is still to be read
+  const bool same = q == out && (n_seqs <= 1 || q_seq == out_seq) && (n_queries <= 1 || q_tok == out_tok) &&
+                    (q_heads <= 1 || q_head == out_head);
+  MI_REQUIRE(same || !outs.meets(RowSet(q, qe, cache->dim).over(n_seqs, q_seq).over(n_queries, q_tok).over(q_heads, q_head)),
+             "mi_hist_attn: out overlaps q without being q");
   hipStream_t s = (hipStream_t) stream;
   switch (cache->dtype) {
     case MI_DT_F32: return launch_attn<MI_DT_F32>(p, plan, cache->dim, workspace, s);

@@ -1106,7 +1106,8 @@ def hist_write(cache, k, v, page_table, lengths, offsets=None, err=None):
 
 def hist_read(cache, page_table, lengths, n_rows=None, offsets=None, dtype=torch.bfloat16, out=None, err=None):
     """The sequences' newest positions as packed rows (k, v) [n_rows, heads, dim], by hist_write's rule.  ``out`` = (k, v)
-    receives them when given (rows that no sequence owns stay as they are there; they are unset otherwise)."""
+    receives them when given (rows that no sequence owns stay as they are there; they are unset otherwise); two tensors
+    or views of one, of any strides, whose rows share no memory."""
     if out is None:
         if n_rows is None:
             raise MiError("hist_read: give n_rows or out")
@@ -1122,7 +1123,8 @@ def hist_read(cache, page_table, lengths, n_rows=None, offsets=None, dtype=torch
 def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
     """Softmax attention of every sequence's new tokens or candidates ``q`` [sequences, heads, dim] or [sequences, tokens,
     heads, dim] over all ``lengths`` positions of its history; the query heads share the cache's heads in equal groups.
-    q: float32 over a float32 cache, bfloat16 otherwise; the result has its shape and type (``out`` may be q itself).  ``scale``: of the scores,
+    q: float32 over a float32 cache, bfloat16 otherwise; the result has its shape and type (``out`` may be
+    q itself, or share no memory with it).  ``scale``: of the scores,
     dim ** -0.5 by default.  A sequence without history gives zeros."""
     n, width, ld_table = _hist_common('hist_attn', cache, page_table, lengths, None, err, q, out)
     shape, dtype, heads, dim = q.shape, q.dtype, cache.n_heads, cache.dim

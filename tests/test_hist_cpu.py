@@ -197,3 +197,48 @@ def test_results_that_overlap_are_refused():
     for os_, kw in (((256, 128, 64), {}), ((128, 0, 64), dict(tokens=1)), ((0, 128, 64), dict(seqs=1))):
         code, msg = attn(os_, **kw)                               # past that check: the workspace is the next
         assert code == -3 and 'workspace' in msg, (os_, kw, msg)
+
+
+def test_results_whose_rows_meet_are_refused():
+    """Rows that share memory across two dimensions, K and V rows in one place, and a result that is partly its own
+    queries: each stride by itself looks right."""
+    from recommendation_amd import _lib
+    lib = _lib.load()
+    base = 1 << 20
+
+    def read(k, v, strides, n=4, offsets=4096):
+        code = lib.mi_hist_read(ctypes.byref(_cache(n_heads=3)), k, v, 1, *strides, n, offsets, 4, 4096, 2, 2, 4096, None, None)
+        return code, lib.mi_last_error().decode()
+
+    far = base << 4
+    for k, v, strides in [
+            (base, base, (192, 64, 192, 64)),                       # the same tensor twice
+            (base, far, (64, 64, 192, 64)), (far, base, (192, 64, 64, 64)),   # row stride = head stride (unfolded)
+            (base, far, (128, 64, 192, 64)), (base, far, (64, 128, 192, 64)),
+            (base, base + 2 * 64, (192, 64, 192, 64)),              # V's heads are K's next heads
+            (base, base + 2 * 192, (192, 64, 192, 64)),             # V's rows are K's next rows
+            (base, base + 2 * 3 * 192, (192, 64, 192, 64)),         # ... the last one only
+            (base + 2 * 3 * 192, base, (192, 64, 192, 64)),
+            (base, base + 16, (384, 64, 384, 64)),                  # half a row apart
+            (base, base, (192, 64, 64, 256))]:                      # the same memory, heads in front in V
+        code, msg = read(k, v, strides)
+        assert code == -1 and 'overlap' in msg, (k, v, strides, code, msg)
+
+    def attn(q, qs, out, os_, tokens=2, seqs=4, heads=2, width=2):
+        code = lib.mi_hist_attn(ctypes.byref(_cache()), q, *qs, heads, tokens, seqs, 4096, width, width, 4096, 0.1, out, *os_, None,
+                                0, None, None)
+        return code, lib.mi_last_error().decode()
+
+    plain = (256, 128, 64)
+    for q, qs, out, os_ in [
+            (far, plain, base, (256, 64, 64)), (far, plain, base, (64, 256, 64)), (far, plain, base, (128, 128, 64)),
+            (far, plain, base, (128, 64, 128)),
+            (base, plain, base, (256, 64, 128)),                    # tokens and heads exchanged
+            (base, plain, base + 2 * 64, plain), (base, plain, base + 2 * 256, plain), (base + 2 * 3 * 256, plain, base, plain),
+            (base, (512, 128, 64), base, plain), (base, (0, 128, 64), base, plain), (base, plain, base + 16, plain)]:
+        code, msg = attn(q, qs, out, os_)
+        assert code == -1 and 'overlap' in msg, (q, qs, out, os_, code, msg)
+    # past every check on the rows of out, the workspace is the next: transposed results, results with gaps
+    for os_ in ((256, 64, 128), (64, 512, 256), (512, 128, 64), (72, 576, 288)):
+        code, msg = attn(far, plain, base, os_, width=65)
+        assert code == -3 and 'workspace' in msg, (os_, code, msg)

@@ -590,6 +590,43 @@ def test_the_result_may_replace_the_queries(dev):
         assert ops.hist_attn(c, q, table, lengths, out=q) is q and torch.equal(q, want)
 
 
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_results_between_each_other_and_between_the_queries(dev, cache):
+    """Results that lie in one buffer with each other or with the queries, and share no row: interleaved by token, by head, heads
+    in front, with gaps of different width."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(41)
+    heads, dim, lens = 2, 64, [40, 0, 100]
+    n, dt = sum(lens), torch.float32 if cache == 'f32' else torch.bfloat16
+    c, table, lengths, t = filled(dev, rng, cache, lens, 16, heads, dim)
+    offs = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int64, device=dev)
+    k, v = ops.hist_read(c, table, lengths, n, offsets=offs, dtype=dt)
+    new = lambda *shape: torch.full(shape, 5.0, dtype=dt, device=dev)
+    a, b, d, e = new(n, 2, heads, dim), new(n, heads, 2, dim), new(2, heads, n, dim), new(n, 2 * heads * dim + heads * 16)
+    half = heads * dim
+    for pair in ((a[:, 0], a[:, 1]), (b[:, :, 1], b[:, :, 0]), (d[0].transpose(0, 1), d[1].transpose(0, 1)),
+                 (e[:, :half].view(n, heads, dim), e[:, half:].view(n, heads, dim + 16)[..., :dim])):
+        ops.hist_read(c, table, lengths, offsets=offs, out=pair)
+        assert torch.equal(pair[0], k) and torch.equal(pair[1], v)
+    assert bool((e[:, half:].view(n, heads, dim + 16)[..., dim:] == 5.0).all())
+    q = torch.from_numpy(rng.standard_normal((3, 2, 4, dim))).to(dev, dt)
+    want = ops.hist_attn(c, q, table, lengths)
+    a, b, d = new(3, 2, 2, 4, dim), new(3, 2, 4, 2, dim), new(3, 4, 2, 2 * dim)
+    views = [(a[:, :, 0], a[:, :, 1]), (a[:, 1], a[:, 0]), (b[..., 1, :], b[..., 0, :]),
+             (d[..., :dim].transpose(1, 2), d[..., dim:].transpose(1, 2))]
+    for mine, out in views:
+        mine.copy_(q)
+        ops.hist_attn(c, mine, table, lengths, out=out)
+        assert torch.equal(out, want) and torch.equal(mine, q)
+    x = new(3, 4, 2, dim).transpose(1, 2)
+    x.copy_(q)
+    assert ops.hist_attn(c, x, table, lengths, out=x) is x and torch.equal(x, want)
+    for bad in (lambda: ops.hist_read(c, table, lengths, offsets=offs, out=(k, k)),
+                lambda: ops.hist_attn(c, q, table, lengths, out=q.view(3, 4, 2, dim).transpose(1, 2))):
+        with pytest.raises(ops.MiError, match='overlap'):
+            bad()
+
+
 def test_two_calls_at_once_on_two_streams(dev):
     """Calls that share nothing but the cache they read run side by side with their own workspaces."""
     from recommendation_amd import ops
