@@ -914,7 +914,7 @@ int mi_parse_records(const char* text, int64_t len, int n_fields, int bag_len, i
  *
  * Pages hold page_size positions of ONE sequence; page_table[b][i] (int32, row stride ld_table, table_width pages of
  * room) names the page of positions [i*page_size, (i+1)*page_size) of sequence b.  Sequences may share pages that
- * nobody writes any more.  lengths[b] (int32) counts the positions of sequence b, those that the same step appends
+ * nobody writes any more, and a call that only reads takes ld_table 0, one row for all of them.  lengths[b] (int32) counts the positions of sequence b, those that the same step appends
  * included; <= 0 is a sequence without history (padding of a batch).
  * MI_IDERR_RANGE is raised for a page id outside [0, n_pages) where a position needs it and for a length beyond
  * table_width*page_size; such positions are skipped (write), zeros (read), absent (attention).
@@ -949,7 +949,8 @@ int mi_hist_read(const mi_hist_cache* cache, void* k, void* v, int dtype, int64_
 
 /* Attention of n_queries new tokens (or candidates) of every sequence over ALL lengths[b] positions of its history:
  *   out[b][t][h] = sum_j softmax_j(scale * <q[b][t][h], k_j>) v_j,   k_j, v_j of cache head h / (q_heads / n_heads).
- * Queries of one sequence do not see each other.  A row without a position of finite score gives zeros.  q, out:
+ * Queries of one sequence do not see each other, and each sees every position: several events of one user, each to see
+ * those up to itself, are sequences of lengths len - n + 1 .. len over the same pages.  A row without a position of finite score gives zeros.  q, out:
  * f32 for an f32 cache, bf16 otherwise; sequence, token and head strides in elements, 16-byte aligned.  out may be q
  * (the same rows in the same places) and must not overlap it otherwise; its own rows must not overlap, as in a read.
  * Sums and softmax statistics in f32; weighted values are summed before they are divided, so values should stay below

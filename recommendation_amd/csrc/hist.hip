@@ -1267,10 +1267,12 @@ int check_cache(const mi_hist_cache* c, const char* who) {
   return MI_OK;
 }
 
-int check_table(const int32_t* table, int64_t ld, int width, const int32_t* lengths, int64_t n_seqs, const char* who) {
+// A call that only reads the pages takes one row of the table for all sequences too (ld 0); in a write they would all append
+// to the same pages.
+int check_table(const int32_t* table, int64_t ld, int width, const int32_t* lengths, int64_t n_seqs, bool write, const char* who) {
   MI_REQUIRE(table && lengths, "%s: null page table or lengths", who);
   MI_REQUIRE(n_seqs >= 0 && n_seqs <= INT32_MAX, "%s: n_seqs %lld", who, (long long) n_seqs);
-  MI_REQUIRE(width >= 1 && (ld >= width || n_seqs <= 1), "%s: page table width %d with row stride %lld", who, width, (long long) ld);
+  MI_REQUIRE(width >= 1 && (ld >= width || n_seqs <= 1 || (ld == 0 && !write)), "%s: page table width %d with row stride %lld", who, width, (long long) ld);
   return MI_OK;
 }
 
@@ -1345,7 +1347,7 @@ int rows_call(const char* who, bool read, const mi_hist_cache* cache, const void
   MI_REQUIRE(dtype == MI_DT_F32 || dtype == MI_DT_BF16, "%s: rows are f32 or bf16, not %d", who, dtype);
   MI_REQUIRE(n_rows >= 0, "%s: n_rows %lld", who, (long long) n_rows);
   if (n_rows == 0 || n_seqs == 0) return MI_OK;
-  if (int rc = check_table(table, ld_table, width, lengths, n_seqs, who)) return rc;
+  if (int rc = check_table(table, ld_table, width, lengths, n_seqs, !read, who)) return rc;
   MI_REQUIRE(k && v, "%s: null rows", who);
   MI_REQUIRE(aligned16(k, dtype == MI_DT_F32 ? 4 : 2, k_row, k_head) && aligned16(v, dtype == MI_DT_F32 ? 4 : 2, v_row, v_head),
              "%s: rows must start on 16-byte boundaries", who);
@@ -1439,7 +1441,7 @@ extern "C" int mi_hist_attn(const mi_hist_cache* cache, const void* q, int64_t q
   MI_REQUIRE(n_queries >= 0 && q_heads >= 1 && q_heads % cache->n_heads == 0,
              "mi_hist_attn: %d queries of %d heads over a cache of %d heads", n_queries, q_heads, cache->n_heads);
   if (n_seqs == 0 || n_queries == 0) return MI_OK;
-  if (int rc = check_table(page_table, ld_table, table_width, lengths, n_seqs, "mi_hist_attn")) return rc;
+  if (int rc = check_table(page_table, ld_table, table_width, lengths, n_seqs, false, "mi_hist_attn")) return rc;
   MI_REQUIRE(q && out, "mi_hist_attn: null q or out");
   const int qe = cache->dtype == MI_DT_F32 ? 4 : 2;
   MI_REQUIRE(aligned16(q, qe, q_seq, q_tok, q_head) && aligned16(out, qe, out_seq, out_tok, out_head),

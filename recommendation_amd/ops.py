@@ -1125,7 +1125,9 @@ def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
     heads, dim] over all ``lengths`` positions of its history; the query heads share the cache's heads in equal groups.
     q: float32 over a float32 cache, bfloat16 otherwise; the result has its shape and type (``out`` may be
     q itself, or share no memory with it).  ``scale``: of the scores,
-    dim ** -0.5 by default.  A sequence without history gives zeros."""
+    dim ** -0.5 by default.  A sequence without history gives zeros.  Every query sees all positions; to attend several
+    new events of a user, each up to itself, make them sequences of their own: ``page_table`` the user's row expanded,
+    ``lengths`` counting up."""
     n, width, ld_table = _hist_common('hist_attn', cache, page_table, lengths, None, err, q, out)
     shape, dtype, heads, dim = q.shape, q.dtype, cache.n_heads, cache.dim
     if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != dim or shape[-2] < 1 or shape[-2] % heads:

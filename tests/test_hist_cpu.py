@@ -242,3 +242,25 @@ def test_results_whose_rows_meet_are_refused():
     for os_ in ((256, 64, 128), (64, 512, 256), (512, 128, 64), (72, 576, 288)):
         code, msg = attn(far, plain, base, os_, width=65)
         assert code == -3 and 'workspace' in msg, (os_, code, msg)
+
+
+def test_one_table_row_for_all_sequences():
+    """Row stride 0 (an expanded table): taken where the pages are only read, refused where they are written."""
+    from recommendation_amd import _lib
+    lib = _lib.load()
+
+    def attn(ld):
+        code = lib.mi_hist_attn(ctypes.byref(_cache()), 1 << 20, 128, 128, 64, 2, 1, 4, 4096, ld, 65, 4096, 0.1, 1 << 21, 128, 128, 64,
+                                None, 0, None, None)
+        return code, lib.mi_last_error().decode()
+
+    code, msg = attn(0)                                              # the workspace is the next check
+    assert code == -3 and 'workspace' in msg
+    for ld in (-65, -1, 1, 64):
+        code, msg = attn(ld)
+        assert code == -1 and 'row stride' in msg, (ld, code, msg)
+    args = (1 << 20, 1 << 21, 1, 128, 64, 128, 64)
+    # more rows than one call can number: the check behind the table's
+    assert lib.mi_hist_read(ctypes.byref(_cache()), *args, 1 << 30, 4096, 4, 4096, 0, 2, 4096, None, None) == -4
+    assert lib.mi_hist_write(ctypes.byref(_cache()), *args, 1 << 30, 4096, 4, 4096, 0, 2, 4096, None, None) == -1
+    assert 'row stride' in lib.mi_last_error().decode()

@@ -547,6 +547,33 @@ def test_histories_grow_event_by_event(dev, cache):
     np.testing.assert_array_equal(values(fresh), values(c))
 
 
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('before', [3, 600, 3000])
+def test_several_events_of_one_user_see_those_before_them(dev, cache, before):
+    """Events appended in one call, each attending up to itself: one sequence per event over the user's expanded table row."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(before)
+    page, heads, dim, new = 16, 2, 64, 5
+    total = before + new
+    c, table, lengths, t = filled(dev, rng, cache, [total], page, heads, dim)
+    k, v = (torch.from_numpy(rng.integers(-7, 8, size=(new, heads, dim))).to(dev, torch.float32) for _ in range(2))
+    ops.hist_write(c, k, v, table, lengths)                                  # whole numbers: exact in every type
+    dt = torch.float32 if cache == 'f32' else torch.bfloat16
+    q = torch.from_numpy(rng.standard_normal((new, 4, dim))).to(dev, dt)
+    rows = table.expand(new, -1)
+    lens = np.arange(before + 1, total + 1)
+    upto = torch.from_numpy(lens.astype(np.int32)).to(dev)
+    got = ops.hist_attn(c, q, rows, upto)
+    assert torch.equal(got, ops.hist_attn(c, q, rows.contiguous(), upto))
+    want, absv, size = oh.attention(values(c), q.double().cpu().numpy()[:, None], np.repeat(t, new, 0), lens, dim ** -0.5, page)
+    held("hist_attn %s events of one user after %d" % (cache, before),
+         (np.abs(got.double().cpu().numpy()[:, None] - want) / bound(cache, dim, total, want, absv, size)).max(), 1.0)
+    k2, v2 = ops.hist_read(c, rows, upto, new, dtype=torch.float32)          # each event's own row
+    assert torch.equal(k2, k) and torch.equal(v2, v)
+    with pytest.raises(ops.MiError, match='row stride'):
+        ops.hist_write(c, k, v, rows, upto)
+
+
 def test_captured_attention_over_long_histories(dev):
     """The two launches and the workspace between them inside graphs: two graphs captured one after the other, replayed in
     turn on two streams with new lengths and queries, eager calls between; every replay equals the eager call."""
