@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from oracle import hist as oh
+from tests import hist_cases
 
 
 def test_oracle_8_bit_rows_by_hand():
@@ -264,3 +265,30 @@ def test_one_table_row_for_all_sequences():
     assert lib.mi_hist_read(ctypes.byref(_cache()), *args, 1 << 30, 4096, 4, 4096, 0, 2, 4096, None, None) == -4
     assert lib.mi_hist_write(ctypes.byref(_cache()), *args, 1 << 30, 4096, 4, 4096, 0, 2, 4096, None, None) == -1
     assert 'row stride' in lib.mi_last_error().decode()
+
+
+@pytest.mark.parametrize('dtype', [0, 1, 2])
+@pytest.mark.parametrize('case', hist_cases.CUTS)
+def test_the_long_cases_take_the_cuts_they_are_for(dtype, case):
+    """More units than workgroups, whole rows or runs that cross them: a change of the rules must not leave them untested."""
+    users, shortest, longest, heads, group, tokens, dim, aligned, run = case
+    lens = hist_cases.lengths_for(np.random.default_rng(users), users, shortest, longest)
+    cut = hist_cases.cut_of(dtype, lens, -(-longest // 16), 16, heads, group, tokens, dim)
+    assert cut['aligned'] == aligned and cut['run'] >= run, cut
+    seen = {(c['RT'], c['NR'], c['NG'] > 1, c['aligned']) for c in (
+        hist_cases.cut_of(dtype, hist_cases.lengths_for(np.random.default_rng(x[0]), *x[:3]), -(-x[2] // 16), 16, *x[3:7])
+        for x in hist_cases.CUTS)}
+    assert {(1, 1, False, True), (2, 2, False, True), (2, 4, True, True), (1, 2, False, True), (1, 1, False, False),
+            (2, 2, False, False), (2, 4, True, False), (1, 4, False, False)} <= seen
+
+
+def test_counting_histories_show_a_lost_tile():
+    """Planted in the sums: without any one position, tile of 16 or unit of 128, some channel is off by more than the bound that
+    the attention is held to (2^-8 of the sum in 16 bits)."""
+    rows, sums = hist_cases.counting_rows(np.random.default_rng(2), 3000, 2, 32)
+    assert np.array_equal(np.cumsum(rows, 0), sums[1:]) and np.abs(sums[:, :, 1:]).max() <= 24
+    bound = np.abs(sums[3000]) * 2.0 ** -8 + 2.0 ** -20
+    for size in (1, 16, 128):
+        for at in range(0, 3000, size):
+            lost = sums[min(at + size, 3000)] - sums[at]
+            assert (np.abs(lost) > bound)[:, 1:].any(1).all(), (size, at)

@@ -14,6 +14,7 @@ import pytest
 import torch
 
 from oracle import hist as oh
+from tests import hist_cases
 from tests.errlog import held
 
 pytestmark = pytest.mark.gpu
@@ -292,6 +293,61 @@ def test_attention_at_every_edge_of_tile_and_page(dev, cache, dim, room):
     ([700, 31, 400], 1, 1, 150, 64, 16), ([300, 290], 2, 1, 40, 128, 32), ([40000, 5], 1, 2, 1, 32, 256)])
 def test_attention_over_long_histories(dev, cache, lens, heads, group, tokens, dim, page):
     run_attn(dev, np.random.default_rng(len(lens) + dim), cache, lens, page, heads, group, tokens, dim)
+
+
+def one_history(dev, rng, cache, k, v, page):
+    """A cache that holds one history of rows k, v, everything else NaN; its page table of one row."""
+    from recommendation_amd import ops
+    n, heads, dim = k.shape
+    width = -(-n // page)
+    c = poisoned(dev, cache, width + 3, page, heads, dim)
+    table = torch.from_numpy(tables(rng, [n], page, width, width + 3)).to(dev)
+    ops.hist_write(c, torch.from_numpy(k).to(dev, torch.float32), torch.from_numpy(v).to(dev, torch.float32), table,
+                   torch.tensor([n], dtype=torch.int32, device=dev))
+    return c, table
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('case', hist_cases.CUTS, ids=lambda x: '-'.join(str(y) for y in x[:7]))
+def test_every_position_counts_once_however_the_work_is_cut(dev, cache, case):
+    """Equal keys: all weights are 1 and all sums whole numbers, exact in f32 in any order, so an element times the length is
+    off by the division (8 u) and in 16 bits by the result's rounding (2^-8) of the sum, and by nothing where that is 0."""
+    from recommendation_amd import ops
+    users, shortest, longest, heads, group, tokens, dim = case[:7]
+    rng = np.random.default_rng(users)
+    lens = hist_cases.lengths_for(rng, users, shortest, longest)
+    rows, sums = hist_cases.counting_rows(rng, longest, heads, dim)
+    k = np.broadcast_to(rng.standard_normal((1, heads, dim)), rows.shape)
+    c, table = one_history(dev, rng, cache, np.ascontiguousarray(k), rows, 16)
+    q = torch.from_numpy(rng.standard_normal((users, tokens, heads * group, dim))).to(dev, torch.float32 if cache == 'f32' else torch.bfloat16)
+    out = ops.hist_attn(c, q, table.expand(users, -1), torch.tensor(lens, dtype=torch.int32, device=dev))
+    n = np.maximum(np.array(lens), 0)
+    want = np.repeat(sums[n], group, 1)[:, None]                              # [users, 1, q heads, dim]
+    got = out.double().cpu().numpy() * n[:, None, None, None]
+    assert (np.abs(got - want) <= np.abs(want) * (8 * U + (0 if cache == 'f32' else 2.0 ** -8))).all()
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('case', hist_cases.CUTS, ids=lambda x: '-'.join(str(y) for y in x[:7]))
+def test_attention_however_the_work_is_cut(dev, cache, case):
+    """Random rows, each history held to its own bound, with the additions that really follow each other in its sums."""
+    from recommendation_amd import ops
+    users, shortest, longest, heads, group, tokens, dim = case[:7]
+    rng = np.random.default_rng(users)
+    lens = hist_cases.lengths_for(rng, users, shortest, longest)
+    k, v = rng.standard_normal((2, longest, heads, dim))
+    c, table = one_history(dev, rng, cache, k, v * np.exp2(rng.integers(-3, 4, size=(longest, heads, 1))), 16)
+    q = torch.from_numpy(rng.standard_normal((users, tokens, heads * group, dim)) * 1.5).to(dev, torch.float32 if cache == 'f32' else torch.bfloat16)
+    out = ops.hist_attn(c, q, table.expand(users, -1), torch.tensor(lens, dtype=torch.int32, device=dev)).double().cpu().numpy()
+    t = np.broadcast_to(table.cpu().numpy(), (users, table.shape[1]))
+    cut = hist_cases.cut_of(ops.HistCache._DTYPES[DTYPES[cache]], lens, t.shape[1], 16, heads, group, tokens, dim)
+    held_values, q = values(c), q.double().cpu().numpy()
+    worst = 0.0
+    for b in range(users):
+        want, absv, size = oh.attention(held_values, q[b:b + 1], t[b:b + 1], lens[b:b + 1], dim ** -0.5, 16)
+        limit = bound(cache, dim, hist_cases.depth_of(cut, max(lens[b], 0)), want, absv, size)
+        worst = max(worst, (np.abs(out[b:b + 1] - want) / limit).max())
+    held("hist_attn %s cut %s run %d" % (cache, '-'.join(str(y) for y in case[:7]), cut['run']), worst, 1.0)
 
 
 @pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
