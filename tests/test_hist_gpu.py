@@ -175,6 +175,67 @@ def test_rows_of_any_stride_and_table_views(dev, cache):
     assert bool((out[:, 0, :, dim:] == 5.0).all()) and bool((out[:, 1, :, :16] == 5.0).all())
 
 
+@pytest.mark.parametrize('cache', ['f32', 'bf16', 'e4m3'])
+def test_captured_strided_writes_touch_their_rows_alone(dev, cache):
+    """Byte for byte over the whole pool: pages of no table, slots behind a history and in front of the appended rows keep
+    what they held, eager and in every replay, with rows of any stride and rows nobody owns among them."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(29)
+    page, heads, dim, n_pages, lens, new = 16, 3, 64, 20, [40, 9, 0, 100], [17, 9, 2, 33]
+    dt = torch.float32 if cache == 'f32' else torch.bfloat16
+    n = sum(new) + 3                                                         # three rows behind the last sequence
+    t = tables(rng, lens, page, 7, n_pages)
+    wide = torch.full((4, 16), 11, dtype=torch.int32, device=dev)
+    wide[:, 5:12] = torch.from_numpy(t).to(dev)
+    table, lengths = wide[:, 5:12], torch.tensor(lens, dtype=torch.int32, device=dev)
+    offs = np.concatenate([[0], np.cumsum(new)]).astype(np.int64)
+    offsets = torch.from_numpy(offs).to(dev)
+    fused = torch.zeros((n, heads * dim + 64), dtype=dt, device=dev)
+    k, v = fused[:, 32:32 + heads * dim].view(n, heads, dim), torch.zeros((heads, n, dim), dtype=dt, device=dev).transpose(0, 1)
+    c = poisoned(dev, cache, n_pages, page, heads, dim)
+    where, bad = oh.places(n, offs, len(lens), t, page, n_pages, lens)
+    assert not bad and 'none' in where and None in where
+    touched = torch.zeros((n_pages, heads, 2, page), dtype=torch.bool)
+    for w in where:
+        if isinstance(w, tuple):
+            touched[w[0], :, :, w[1]] = True
+    touched = touched.to(dev)
+
+    def clear():
+        c.kv.view(torch.uint8).fill_(0xff)                                   # NaN in every type
+        if cache == 'e4m3':
+            c.exps.fill_(255)
+
+    def check(rows):
+        kept = c.kv.view(torch.uint8).view(n_pages, heads, 2, page, -1)[~touched]
+        assert bool((kept == 0xff).all()) and (cache != 'e4m3' or bool((c.exps[~touched] == 255).all()))
+        want = rows if cache == 'f32' else torch.from_numpy(rows).to(torch.bfloat16).double().numpy()
+        if cache == 'e4m3':
+            want = oh.quantise(want)[0]
+        full = values(c)
+        for i, w in enumerate(where):
+            if isinstance(w, tuple):
+                np.testing.assert_array_equal(full[w[0], :, :, w[1]], want[i].transpose(1, 0, 2))
+
+    def draw():
+        rows = rng.standard_normal((n, 2, heads, dim)).astype(np.float32).astype(np.float64)
+        k.copy_(torch.from_numpy(rows[:, 0]))
+        v.copy_(torch.from_numpy(rows[:, 1]))
+        clear()
+        return rows
+
+    rows = draw()
+    ops.hist_write(c, k, v, table, lengths, offsets=offsets)
+    check(rows)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.hist_write(c, k, v, table, lengths, offsets=offsets)
+    for _ in range(3):
+        rows = draw()
+        g.replay()
+        check(rows)
+
+
 def test_rows_without_a_place(dev):
     """Lengths shorter than the rows given, padded sequences, bad pages and histories beyond the table."""
     from recommendation_amd import ops
@@ -539,6 +600,55 @@ def test_infinite_and_nan_values(dev, cache):
     size = np.where(np.isfinite(size), size, 64.0)
     err = (np.abs(got[1].double().cpu().numpy() - want[1]) / bound(cache, 64, 40, want, absv, size)[1]).max()
     held("hist_attn %s one -inf score" % cache, err, 1.0)
+
+
+@pytest.mark.parametrize('dim', [32, 128])
+@pytest.mark.parametrize('lens', [[40, 40, 40, 40], [700, 40, 600, 700], [1500, 40, 1400, 1500]])
+def test_nan_codes_in_an_8_bit_cache(dev, lens, dim):
+    """Written as infinities and NaN: a NaN in a live key makes the row's result NaN, one in a live value its channel; behind
+    the history, in dead slots of the last page, neither they nor exponent bytes of 255 are seen."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(33)
+    c, table, lengths, t = filled(dev, rng, 'e4m3', lens, 16, 2, dim)
+    q = torch.from_numpy(rng.standard_normal((4, 1, 4, dim))).to(dev, torch.bfloat16)
+    clean = ops.hist_attn(c, q, table, lengths)
+    assert torch.isfinite(clean).all()                                       # the rest of the cache is NaN
+    offs = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int64, device=dev)
+    k, v = ops.hist_read(c, table, lengths, sum(lens), offsets=offs, dtype=torch.float32)
+    at = np.concatenate([[0], np.cumsum(lens)])
+    k[int(at[1]) + 21, 0, 5] = float('inf')                                  # user 1, head 0: a key
+    v[int(at[2]) + lens[2] - 1, 1, 7] = float('nan')                         # user 2, head 1: channel 7 of the newest value
+    v[int(at[2]) + 3, 1, 9] = -float('inf')
+    ops.hist_write(c, k, v, table, lengths, offsets=offs)
+    got = ops.hist_attn(c, q, table, lengths)
+    want = clean.clone()
+    want[1, :, :2] = float('nan')
+    want[2, :, 2:, 7] = want[2, :, 2:, 9] = float('nan')
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    keep = ~torch.isnan(want)
+    assert torch.equal(got[keep], clean[keep])
+    shorter = lengths - torch.tensor([0, 20, 1, 0], dtype=torch.int32, device=dev)   # user 2's newest row is dead now
+    got = ops.hist_attn(c, q, table, shorter)
+    assert not torch.isnan(got[1]).any() and not torch.isnan(got[2, :, :, 7]).any() and torch.isnan(got[2, :, 2:, 9]).all()
+
+
+@pytest.mark.parametrize('cache', ['f32', 'bf16'])
+@pytest.mark.parametrize('lens', [[40, 33], [700, 600], [1500, 1300]])
+def test_an_infinite_score_shows_as_nan(dev, cache, lens):
+    """+inf - +inf: the whole result of that query head is NaN, early or late in the history, the other user's is not touched."""
+    from recommendation_amd import ops
+    rng = np.random.default_rng(34)
+    c, table, lengths, t = filled(dev, rng, cache, lens, 16, 1, 64)
+    q = torch.from_numpy(rng.standard_normal((2, 1, 2, 64))).to(dev, DTYPES[cache])
+    q[:, :, :, 0] = 1.0
+    clean = ops.hist_attn(c, q, table, lengths)
+    for pos in (0, 17, lens[0] - 1):
+        held_key = c.kv[int(t[0][pos // 16]), 0, 0, pos % 16, 0].clone()
+        c.kv[int(t[0][pos // 16]), 0, 0, pos % 16, 0] = float('inf')
+        got = ops.hist_attn(c, q, table, lengths)
+        assert torch.isnan(got[0]).all() and torch.equal(got[1], clean[1])
+        c.kv[int(t[0][pos // 16]), 0, 0, pos % 16, 0] = held_key
+    assert torch.equal(ops.hist_attn(c, q, table, lengths), clean)
 
 
 # ------------------------------------------------------------------------------------------------ used together
