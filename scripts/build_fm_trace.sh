@@ -36,7 +36,7 @@ f=f.replace("  // combine the field phases (lanes that own the same columns)\n",
 f=f.replace("  float tot = pair + lin;\n","  float tot = pair + lin;\n  TS_MARK(3);\n",1)
 open('fm_body.h','w').write(f)
 P
-/opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -Wall -Wno-unused-function -DTS_TRACE -I. -I../../../recommendation_amd/csrc -c fm.hip -o fm_ts.o
+/opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops -DTS_TRACE -I. -I../../../recommendation_amd/csrc -c fm.hip -o fm_ts.o
 cd ../../../recommendation_amd/csrc
 /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o ../../scripts/exp/libmi_tstrace.so $(ls *.o | grep -v '^fm.o$') ../../scripts/exp/l1/fm_ts.o -ldl
 echo built

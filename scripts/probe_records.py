@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Read-modify-write rate of sorted distinct 256-byte FM records, and the forward's gather rate, by access shape.
-Build: hipcc --offload-arch=gfx950 -O3 -shared -fPIC scripts/rec_probe.hip -o scripts/exp/librecprobe.so
+Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -shared -fPIC scripts/rec_probe.hip -o scripts/exp/librecprobe.so
 usage: probe_records.py [rows_millions=33.76]"""
 import ctypes
 import os

@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Random-segment read rate of the HBM as a function of segment size: the ceiling of a row gather at
-that row width.  Build: hipcc --offload-arch=gfx950 -O3 -shared -fPIC scripts/seg_probe.hip -o scripts/exp/libsegprobe.so
+that row width.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -shared -fPIC scripts/seg_probe.hip -o scripts/exp/libsegprobe.so
 usage: probe_segments.py [table_GiB=8] [GiB_read_per_launch=2]"""
 import ctypes
 import os

@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Read-modify-write rate of sorted distinct 512-byte rows with a per-row fp32 state word, by where the word lives.
-Build: hipcc --offload-arch=gfx950 -O3 -shared -fPIC scripts/wide_probe.hip -o scripts/exp/libwideprobe.so
+Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -shared -fPIC scripts/wide_probe.hip -o scripts/exp/libwideprobe.so
 usage: probe_wide_rows.py [rows_millions=125]"""
 import ctypes
 import os
