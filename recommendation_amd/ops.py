@@ -1090,7 +1090,7 @@ def _hist_rows_call(name, what, cache, k, v, page_table, lengths, offsets, err):
         raise MiError("%s: %d rows do not divide among %d sequences (pass offsets)" % (what, rows, n))
     if rows <= 1 or shape[1] == 1:  # a dimension of one entry is never stepped over: its stride says nothing
         ks, vs = ([0 if shape[d] <= 1 else st[d] for d in range(2)] for st in (ks, vs))
-    _lib.call(name, cache._ref, k.data_ptr(), v.data_ptr(), MI_DT_BF16 if dtype is torch.bfloat16 else MI_DT_F32, ks[0], ks[1],
+    _lib.call(name, cache.ref(), k.data_ptr(), v.data_ptr(), MI_DT_BF16 if dtype is torch.bfloat16 else MI_DT_F32, ks[0], ks[1],
               vs[0], vs[1], rows, offsets.data_ptr() if offsets is not None else None, n, page_table.data_ptr(), ld_table,
               width, lengths.data_ptr(), err.data_ptr() if err is not None else None, _hist_stream(cache._index))
 
@@ -1151,9 +1151,9 @@ def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
     if n <= 1 or shape[-2] == 1 or tokens == 1:
         sizes = (n, tokens, shape[-2])
         qs, os_ = ([st[d] if sizes[d] > 1 else 0 for d in range(3)] for st in (qs, os_))
-    ws_bytes = _lib.load().mi_hist_attn_workspace_bytes(cache._ref, n, tokens, shape[-2], width)
+    ws_bytes = _lib.load().mi_hist_attn_workspace_bytes(cache.ref(), n, tokens, shape[-2], width)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-    _lib.call('mi_hist_attn', cache._ref, q.data_ptr(), qs[0], qs[1], qs[2], shape[-2], tokens, n, page_table.data_ptr(),
+    _lib.call('mi_hist_attn', cache.ref(), q.data_ptr(), qs[0], qs[1], qs[2], shape[-2], tokens, n, page_table.data_ptr(),
               ld_table, width, lengths.data_ptr(), cache._scale if scale is None else scale, out.data_ptr(), os_[0], os_[1],
               os_[2], ws.data_ptr() if ws is not None else None, ws_bytes, err.data_ptr() if err is not None else None,
               _hist_stream(cache._index))
