@@ -917,11 +917,13 @@ int mi_parse_records(const char* text, int64_t len, int n_fields, int bag_len, i
  * nobody writes any more, and a call that only reads takes ld_table 0, one row for all of them.  lengths[b] (int32) counts the positions of sequence b, those that the same step appends
  * included; <= 0 is a sequence without history (padding of a batch).
  * MI_IDERR_RANGE is raised for a page id outside [0, n_pages) where a position needs it and for a length beyond
- * table_width*page_size; such positions are skipped (write), zeros (read), absent (attention).
+ * table_width*page_size; such positions are skipped (write), zeros (read), absent (attention).  The memory that a call
+ * writes (pages of a write, rows of a read or attention) must not be memory that it reads, but for out == q.
  * ---------------------------------------------------------------------------------- */
 typedef struct mi_hist_cache {
   void* kv;        /* [n_pages][n_heads][2][page_size][dim], 0 keys, 1 values; 16-byte aligned */
-  uint8_t* exps;   /* e4m3 only: [n_pages][n_heads][2][page_size]; a row stands for code * 2^(exps - 127) */
+  uint8_t* exps;   /* e4m3 only: [n_pages][n_heads][2][page_size]; a row stands for code * 2^(exps - 127), exps 1..254
+                      (a write leaves 1..247; 0 makes a row zeros, 255 is no number) */
   int64_t n_pages;
   int n_heads;
   int page_size;   /* a power of two, 16..1024 */

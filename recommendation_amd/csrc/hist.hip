@@ -362,8 +362,8 @@ __global__ __launch_bounds__(256) void hist_rows_kernel(RowArgs p, int token_shi
 template <int CT, int IT, bool READ>
 int launch_rows(const RowArgs& p, int dim, hipStream_t s) {
   // at least the rows of one instruction; beyond that up to four tokens a wave as long as there are four waves for every
-  // SIMD.  f32 rows leave a wave token by token: 8 KB at a time then (65 k rows of 8 x 128 read back: 103 us, 119 with
-  // four tokens a wave; in bf16 287 and 280, written from bf16 102 and 88).
+  // SIMD.  f32 rows leave a wave token by token: 8 KB at a time then (65 k rows of 8 x 128 read back from e4m3 in f32: 134 us
+  // so, 152 with four tokens a wave; 250 k rows in bf16: 286 token by token, 281 with four; 65 k written from bf16: 106, 91).
   const int groups = 64 / (dim / 8);
   int shift = 0;
   while ((2 * p.H) << shift < groups && shift < 6) ++shift;
@@ -405,7 +405,10 @@ struct AttnArgs {
   int32_t* err;
 };
 
-// Waves on a SIMD, asked of the compiler (registers) and counted on when the work is cut.
+// Waves on a SIMD, asked of the compiler (registers) and counted on when the work is cut.  256 channels run one: two would fit
+// in 8 bits (215-226 registers), would spill 4-25 in 16 bits and need 480 and more in f32.  Calls over long histories do not
+// feel it (see Wave); calls where a workgroup has a history of up to a thousand positions and lengths differ do: 547 MB in
+// bf16 171 us, the same bytes at 128 channels 114.
 constexpr int split_waves(bool f32, int dim, int RT) {
   return dim == 256 ? 1 : dim == 128 ? (f32 ? 3 - RT : 4 - RT) : dim == 64 ? (f32 ? 3 : 4) - (RT - 1) : 4 - (RT - 1);
 }
@@ -419,8 +422,9 @@ constexpr int split_waves(bool f32, int dim, int RT) {
 // operand takes output channels j of 16 lanes' 16-byte pieces of a V row, whatever those channels are called.  So no
 // score, probability or value crosses lanes; only the row maximum and sum do (over the four g).
 //
-// What bounds it: the cache's bytes (1 to 16 query rows a head: 6.2-6.7 TB/s over long histories), and from two row tiles
-// on the vector instructions (e4m3, 64 rows: 62 % of the issue slots).
+// What bounds it: the cache's bytes (1 to 16 query rows a head: 6.1-6.7 TB/s in calls that read 0.7-3.2 GB, at 128 and 256
+// channels; 3.1-4.1 in calls that read 80-310 MB), and from two row tiles on the vector instructions (e4m3, 64 rows: two waves
+// a SIMD issue them in 67 % of the cycles).
 template <int DT, int D, int RT, bool STREAM>
 struct Wave {
   static constexpr bool F32 = DT == MI_DT_F32;
@@ -831,7 +835,8 @@ __device__ __forceinline__ int64_t clamped_length(const AttnArgs& p, int32_t len
 }
 
 // Short histories: one wave per (sequence, cache head, RT tiles of 16 query rows).  Through the caches whatever the pool's
-// size: the waves of further row tiles come right behind (35 rows over 27 positions: 149 us so, 187 past them).
+// size: the waves of further row tiles come right behind (35 rows over up to 27 positions: 123 us so, 130 past them; one row
+// over up to 111: 62 and 64; three rows over 22-44: 102 and 100).
 template <int DT, int D, int RT>
 __global__ __launch_bounds__(256, split_waves(DT == MI_DT_F32, D, RT)) void hist_attn_short_kernel(AttnArgs p, int n_tiles) {
   typedef Wave<DT, D, RT, false> W;
@@ -935,7 +940,7 @@ constexpr unsigned int UNIT = 128;
 // Runs of up to ALIGN_RUN units begin and end with a row of work instead, where the chip can hold them all: a second row
 // in a workgroup costs it a second start (lengths, pages, queries, the first positions: some 6 us), more than the uneven
 // pieces do.  A unit is then that many times longer, and a run one unit.  (16 candidates each for 32 users: 38 us with
-// runs that cross rows, 35 so.)
+// runs that cross rows, 35-36 so.)
 constexpr unsigned int ALIGN_RUN = 8;
 
 struct SplitArgs {
@@ -1229,9 +1234,9 @@ int launch_split(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) 
 template <int DT, int D>
 int launch_attn_dim(const AttnArgs& p, const AttnPlan& q, void* ws, hipStream_t s) {
   if (q.short_rows) return launch_short<DT, D>(p, q, s);
-  // past the caches where the pool does not fit the last one (64 bf16 histories of 8-16 k: 479 us so, 537 through them;
-  // the other way round 72 MB of candidates' histories: 57 against 48) and no second row tile reads the same positions
-  // (16 candidates each for 256 users: 199 us past the caches, 165 through them)
+  // past the caches where the pool does not fit the last one (64 bf16 histories of 8-16 k: 470 us so, 523 through them; the
+  // other way round a pool of 164 MB that the call before has read: 38 against 34) and no second row tile reads the same
+  // positions (16 candidates each for 256 users: 203 us past the caches, 174 through them)
   const bool stream = ((int64_t) p.n_pages * p.H * 2 << p.page_shift) * D * Elem<DT>::BYTES > LAST_LEVEL_BYTES &&
                       q.NR == 1 && q.NG == 1;
   return stream ? launch_split<DT, D, true>(p, q, ws, s) : launch_split<DT, D, false>(p, q, ws, s);

@@ -1001,7 +1001,7 @@ class DinUnit(object):
 class HistCache(object):
     """struct mi_hist_cache: pages of keys and values, ``kv`` [n_pages, n_heads, 2, page_size, dim] (0 keys, 1 values) in
     float32, bfloat16 or float8_e4m3fn; an 8-bit cache has ``exps`` [n_pages, n_heads, 2, page_size] beside it (a row
-    stands for code * 2^(exps - 127)).  Which page holds which positions of which sequence is the caller's table."""
+    stands for code * 2^(exps - 127), exps 1 to 254).  Which page holds which positions of which sequence is the caller's table."""
 
     _DTYPES = {torch.float32: MI_DT_F32, torch.bfloat16: MI_DT_BF16, torch.float8_e4m3fn: MI_DT_E4M3}
 
@@ -1127,7 +1127,8 @@ def hist_attn(cache, q, page_table, lengths, scale=None, out=None, err=None):
     q itself, or share no memory with it).  ``scale``: of the scores,
     dim ** -0.5 by default.  A sequence without history gives zeros.  Every query sees all positions; to attend several
     new events of a user, each up to itself, make them sequences of their own: ``page_table`` the user's row expanded,
-    ``lengths`` counting up."""
+    ``lengths`` counting up.  Values should stay below 2^100 in size (they are summed before they are divided), those of an
+    8-bit cache above 2^-100 (their weights are bf16)."""
     n, width, ld_table = _hist_common('hist_attn', cache, page_table, lengths, None, err, q, out)
     shape, dtype, heads, dim = q.shape, q.dtype, cache.n_heads, cache.dim
     if len(shape) not in (3, 4) or shape[0] != n or shape[-1] != dim or shape[-2] < 1 or shape[-2] % heads:

@@ -236,6 +236,25 @@ def test_captured_strided_writes_touch_their_rows_alone(dev, cache):
         check(rows)
 
 
+def test_every_code_and_exponent_byte_of_an_8_bit_cache(dev):
+    """A pool that the caller filled: each of the 256 codes under bytes from 0 (a row of zeros) to 254, in 64 bits rounded once."""
+    from recommendation_amd import ops
+    page, dim = 16, 256
+    c = poisoned(dev, 'e4m3', 1, page, 1, dim)
+    codes = torch.arange(256, dtype=torch.uint8, device=dev)
+    c.kv.view(torch.uint8)[:] = codes
+    each = torch.tensor([0, 1, 2, 3, 60, 100, 118, 126, 127, 128, 140, 200, 246, 247, 253, 254], dtype=torch.uint8, device=dev)
+    c.exps[:] = each
+    table, lengths = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.tensor([16], dtype=torch.int32, device=dev)
+    want = codes.view(torch.float8_e4m3fn).double()[None] * torch.exp2(each.double() - 127)[:, None]
+    want[0] = torch.where(torch.isnan(want[0]), want[0], 0.0)
+    for dtype in (torch.float32, torch.bfloat16):
+        k, v = ops.hist_read(c, table, lengths, 16, dtype=dtype)
+        w = want.to(torch.float32).to(dtype)                                 # the f32 product is exact or infinite
+        for x in (k, v):
+            np.testing.assert_array_equal(x[:, 0].float().cpu().numpy(), w.float().cpu().numpy())
+
+
 def test_rows_without_a_place(dev):
     """Lengths shorter than the rows given, padded sequences, bad pages and histories beyond the table."""
     from recommendation_amd import ops
