@@ -1001,7 +1001,8 @@ class DinUnit(object):
 class HistCache(object):
     """struct mi_hist_cache: pages of keys and values, ``kv`` [n_pages, n_heads, 2, page_size, dim] (0 keys, 1 values) in
     float32, bfloat16 or float8_e4m3fn; an 8-bit cache has ``exps`` [n_pages, n_heads, 2, page_size] beside it (a row
-    stands for code * 2^(exps - 127), exps 1 to 254).  Which page holds which positions of which sequence is the caller's table."""
+    stands for code * 2^(exps - 127), exps 1 to 254).  Which page holds which positions of which sequence is the caller's table.
+    Serving state: the calls over it have no gradients."""
 
     _DTYPES = {torch.float32: MI_DT_F32, torch.bfloat16: MI_DT_BF16, torch.float8_e4m3fn: MI_DT_E4M3}
 
